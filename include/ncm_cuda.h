@@ -527,6 +527,160 @@ NCM_API int ncm_rvq_level_noalloc(float* residual, const uint16_t* codebook, con
  * NCM_ETIMEOUT or NCM_ERANGE accordingly. Allocates nothing. */
 NCM_API int ncm_rvq_level_noalloc_status(ncm_stream_t stream, int32_t* flags);
 
+/* ---------------------------- decode steps: rotary rows, paged cache, drafted
+ * tokens over it, logit rules. None of them has a counterpart in the
+ * reference, whose forward recomputes every position on each call
+ * (src/decoder.zig:50-58); the arithmetic they stand beside is cited. They
+ * keep no state in the context and take no workspace from it, so calls on
+ * different streams, and captured graphs replayed at the same time, do not
+ * share anything but the buffers that the caller passes. They restore the
+ * calling thread's current device. */
+
+/* Rotary positions of `heads` heads side by side in each row (the Q and K
+ * columns of fused QKV rows, say): row t of x starts at x + t * x_stride
+ * (elements) and holds heads * head_dim bf16 values; y likewise. Row t is
+ * rotated by row positions[t] of the tables cos_t / sin_t [table_rows,
+ * rotary_dim] f32, built as ncm_rope_tables_host(head_dim = rotary_dim) or its
+ * Llama 3 form builds them for positions 0, 1, ... (only the first rotary_dim / 2
+ * columns are read). Pair i < rotary_dim / 2 of a head is (x[i],
+ * x[i + rotary_dim / 2]), or (x[2i], x[2i + 1]) with `interleaved`:
+ *   (a, b) -> (a c - b s, b c + a s)
+ * in f32, rounded once to bf16 (rotate_head's bf16 mode rounds every product,
+ * packages/kernels/root.zig:615-633; ncm_attention_bf16 keeps that). `inverse`
+ * rotates by the negative angle: the gradient of the forward rotation.
+ * Columns rotary_dim .. head_dim are copied. y may be x with the same
+ * stride (in place); other overlaps are refused. A position outside
+ * [0, table_rows) makes ncm_sync report NCM_ERANGE and leaves its row
+ * unwritten. rotary_dim even, <= head_dim <= 1024; any alignment of whole elements. */
+NCM_API int ncm_rope_bf16(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride, uint16_t* y, int64_t y_stride,
+                          const int32_t* positions, const float* cos_t, const float* sin_t, int64_t table_rows,
+                          int64_t T, int32_t heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved,
+                          int32_t inverse, ncm_stream_t stream);
+
+/* One layer's paged key/value cache in caller-owned device memory. Pools k and
+ * v are [num_pages, kv_heads, page_size, head_dim] of bf16 bits, int8 or e4m3
+ * codes; the quantised formats keep one f32 scale per (page, head, slot) in
+ * k_scale / v_scale [num_pages, kv_heads, page_size] (NULL for bf16). head_dim
+ * 64 or 128, page_size a power of two from 8 to 1024, num_pages * kv_heads *
+ * page_size < 2^31. */
+enum { NCM_KV_BF16 = 0, NCM_KV_INT8 = 1, NCM_KV_E4M3 = 2 };
+typedef struct ncm_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t format;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int64_t num_pages;
+} ncm_kv_cache_t;
+
+/* The sequences of one call (device arrays). Their new tokens are packed:
+ * rows token_start[b] .. token_start[b + 1] of the call's row arrays, which
+ * hold `rows` rows (rows behind token_start[batch] are left alone). kv_lens[b] counts
+ * the sequence's keys, its new tokens (the last ones) included. Position p is
+ * slot p % page_size of page page_table[b * table_stride + p / page_size];
+ * table_width entries per sequence may be read. A sequence whose numbers do
+ * not fit (a negative count, more new tokens than keys, rows or keys past
+ * the end) is skipped, a page outside [0, num_pages) is not touched, and both make
+ * ncm_sync report NCM_ERANGE. */
+typedef struct ncm_kv_batch {
+  const int32_t* token_start; /* [batch + 1] */
+  const int32_t* kv_lens;     /* [batch] */
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t batch;
+  int64_t rows;
+} ncm_kv_batch_t;
+
+/* Writes the new tokens' rows into the cache: k and v rows [rows, kv_heads *
+ * head_dim] bf16 (row strides in elements, multiples of 8; 16-byte aligned, so the K
+ * and V columns of fused QKV rows serve). Row i of sequence b becomes position
+ * kv_lens[b] - n_b + i. Quantised, per token and head, with A = max |x|:
+ *   int8: code = round(127 x / A), scale = A / 127
+ *   e4m3: code = e4m3(448 x / A),  scale = A / 448
+ * nearest, ties to even, exactly as in real arithmetic; A = 0 stores zeros
+ * with scale 1, and a row holding a NaN or an infinity stores zeros with scale
+ * NaN (it reads back as NaN). Two positions that the page tables map to one
+ * slot leave one of the two there, and not always the same one. */
+NCM_API int ncm_kv_cache_append(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                                const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                                ncm_stream_t stream);
+
+/* Reads positions back as bf16 rows (code * scale, rounded once): row i of
+ * sequence b is position begin[b] + i (begin NULL: 0), i < token_start[b + 1] -
+ * token_start[b]; batch->kv_lens is not used (may be NULL). k and v rows as in
+ * ncm_kv_cache_append: with the K and V columns of fused QKV rows as targets
+ * they are ncm_attention_bf16's operands. */
+NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                                const int32_t* begin, uint16_t* k, int64_t k_stride, uint16_t* v, int64_t v_stride,
+                                ncm_stream_t stream);
+
+/* Attention of each sequence's new tokens ("nodes": one decoded token, a chain
+ * or a tree of drafted tokens) over the cache, which holds them already
+ * (ncm_kv_cache_append). Node i sees every key in front of the nodes, and node
+ * j when bit j % 32 of tree_mask[row * mask_words + j / 32] is set (its own bit
+ * included; row = token_start[b] + i; missing words are zeros); tree_mask NULL: a chain, j <= i.
+ *   out = sum_k softmax_k(scale q . k) v_k    lse = log sum_k exp(scale q . k)
+ * per query head (head h reads kv head h / (heads / kv_heads), as
+ * ncm_attention_bf16 does); a node that sees nothing gets zeros and -inf. q and
+ * out [rows, heads * head_dim] bf16 (row strides in elements, multiples of 8;
+ * 16-byte aligned), lse [rows, heads] f32 or NULL. max_nodes bounds every
+ * sequence's new tokens (at most 1024; a sequence with more is skipped with
+ * NCM_ERANGE) and heads / kv_heads is at most 64. Scores, softmax and sums are f32; the
+ * probabilities are rounded to bf16 for their product with the values. The
+ * result does not depend on how the keys are split over the GPU beyond f32 rounding,
+ * and is the same on every run. `workspace` (16-byte aligned device memory) of
+ * ncm_tree_attention_workspace bytes carries partial sums within the call. */
+NCM_API int ncm_tree_attention_workspace(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                                         int32_t heads, int32_t max_nodes, uint64_t* bytes);
+NCM_API int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                               const uint16_t* q, int64_t q_stride, const uint32_t* tree_mask, int32_t mask_words,
+                               int32_t heads, int32_t max_nodes, float scale, uint16_t* out, int64_t out_stride,
+                               float* lse, void* workspace, uint64_t workspace_bytes, ncm_stream_t stream);
+
+/* Rules on next-token logits, all optional (NULL). Row r owns tokens
+ * token_start[r] .. token_start[r + 1] of `tokens` (num_tokens entries): its prompt (the
+ * first prompt_lens[r]; NULL: none) and what it produced since. In this order:
+ *   repetition[r] (> 0): logits of tokens seen at all: l > 0 ? l / rep : l * rep
+ *   frequency[r], presence[r]: l -= frequency * count + presence * [count > 0],
+ *     count = how often the token was produced (the prompt does not count)
+ *   bias entries bias_start[r] .. bias_start[r + 1] of bias_ids / bias
+ *     (num_bias entries): l += bias; a repeated id adds each of its entries in order
+ *   allowed: bit masks [allowed_count, ceil(vocab / 32)] with row stride
+ *     allowed_stride words; row r uses mask allowed_rows[r] (NULL: mask r;
+ *     -1: none); a token whose bit is 0 becomes -inf, whatever it was.
+ * A token id outside [0, vocab), or list bounds or a mask row outside their
+ * array, is ignored and makes ncm_sync report NCM_ERANGE. */
+typedef struct ncm_logit_rules {
+  const int32_t* tokens;
+  const int32_t* token_start; /* [rows + 1] */
+  int64_t num_tokens;
+  const int32_t* prompt_lens; /* [rows] */
+  const float* repetition;    /* [rows] */
+  const float* frequency;     /* [rows] */
+  const float* presence;      /* [rows] */
+  const int32_t* bias_ids;
+  const float* bias;
+  const int32_t* bias_start; /* [rows + 1] */
+  int64_t num_bias;
+  const uint32_t* allowed;
+  int64_t allowed_stride;
+  int64_t allowed_count;
+  const int32_t* allowed_rows; /* [rows] */
+} ncm_logit_rules_t;
+
+/* out = the rules applied to logits [rows, vocab] (NCM_DTYPE_F32 or
+ * NCM_DTYPE_BF16, row strides in elements), computed in f32. out_dtype is
+ * NCM_DTYPE_F32, or NCM_DTYPE_BF16 for bf16 logits. out may be logits (same type and
+ * stride: in place); other overlaps are refused. Rows are what
+ * ncm_tied_head_logits or a language-model head wrote. */
+NCM_API int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dtype, int64_t stride, void* out,
+                               int32_t out_dtype, int64_t out_stride, int64_t rows, int64_t vocab,
+                               const ncm_logit_rules_t* rules, ncm_stream_t stream);
+
 /* ------------------------------------------------------- measurement */
 
 /* Benchmark instrumentation (no reference counterpart: ncmorph has no timing
@@ -536,7 +690,8 @@ NCM_API int ncm_rvq_level_noalloc_status(ncm_stream_t stream, int32_t* flags);
  * and launch count of one family since the last read, and resets them.
  * Families: "rvq_argmin", "rvq_apply", "linear_bf16", "rvq_decode",
  * "code_sqnorm", "pool_avg", "scale_update", "cast", "attention",
- * "decoder_elementwise", "conv_k3", "upsample"; "*" = all of them. */
+ * "decoder_elementwise", "conv_k3", "upsample", "kv_cache", "logits"; "*" = all
+ * of them. */
 NCM_API int ncm_profile_enable(ncm_ctx_t* ctx, int on);
 NCM_API int ncm_profile_read(ncm_ctx_t* ctx, const char* kernel, double* total_ms, int64_t* launches);
 

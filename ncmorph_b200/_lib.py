@@ -106,6 +106,58 @@ class DecoderWeights(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """Mirror of ncm_kv_cache_t."""
+
+    _fields_ = [
+        ("k", c_vp),
+        ("v", c_vp),
+        ("k_scale", c_vp),
+        ("v_scale", c_vp),
+        ("format", c_i32),
+        ("kv_heads", c_i32),
+        ("head_dim", c_i32),
+        ("page_size", c_i32),
+        ("num_pages", c_i64),
+    ]
+
+
+class KvBatch(ctypes.Structure):
+    """Mirror of ncm_kv_batch_t."""
+
+    _fields_ = [
+        ("token_start", c_vp),
+        ("kv_lens", c_vp),
+        ("page_table", c_vp),
+        ("table_stride", c_i64),
+        ("table_width", c_i32),
+        ("batch", c_i32),
+        ("rows", c_i64),
+    ]
+
+
+class LogitRules(ctypes.Structure):
+    """Mirror of ncm_logit_rules_t."""
+
+    _fields_ = [
+        ("tokens", c_vp),
+        ("token_start", c_vp),
+        ("num_tokens", c_i64),
+        ("prompt_lens", c_vp),
+        ("repetition", c_vp),
+        ("frequency", c_vp),
+        ("presence", c_vp),
+        ("bias_ids", c_vp),
+        ("bias", c_vp),
+        ("bias_start", c_vp),
+        ("num_bias", c_i64),
+        ("allowed", c_vp),
+        ("allowed_stride", c_i64),
+        ("allowed_count", c_i64),
+        ("allowed_rows", c_vp),
+    ]
+
+
 # name -> argtypes (all functions return int status unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "ncm_ctx_create": [ctypes.c_int, ctypes.POINTER(c_vp)],
@@ -165,6 +217,15 @@ SIGNATURES: dict[str, list] = {
     "ncm_conv1d_k3": [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp, ctypes.c_float, ctypes.c_float,
                       c_vp],
     "ncm_post_upsample_conv_host_f32": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64],
+    "ncm_rope_bf16": [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32,
+                      c_vp],
+    "ncm_kv_cache_append": [c_vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), c_vp, c_i64, c_vp, c_i64, c_vp],
+    "ncm_kv_cache_gather": [c_vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), c_vp, c_vp, c_i64, c_vp, c_i64, c_vp],
+    "ncm_tree_attention_workspace": [c_vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), c_i32, c_i32,
+                                     ctypes.POINTER(ctypes.c_uint64)],
+    "ncm_tree_attention": [c_vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), c_vp, c_i64, c_vp, c_i32, c_i32, c_i32,
+                           ctypes.c_float, c_vp, c_i64, c_vp, c_vp, ctypes.c_uint64, c_vp],
+    "ncm_logits_process": [c_vp, c_vp, c_i32, c_i64, c_vp, c_i32, c_i64, c_i64, c_i64, ctypes.POINTER(LogitRules), c_vp],
 }
 _RESTYPES = {"ncm_status_string": ctypes.c_char_p, "ncm_last_error": ctypes.c_char_p}
 

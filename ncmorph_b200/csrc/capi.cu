@@ -62,7 +62,7 @@ namespace ncm {
 const char* const kKernelNames[KID_COUNT] = {"rvq_argmin", "rvq_apply",    "linear_bf16", "rvq_decode",
                                              "code_sqnorm", "pool_avg",     "scale_update", "cast",
                                              "attention",   "decoder_elementwise", "conv_k3",
-                                             "upsample"};
+                                             "upsample",    "kv_cache",     "logits"};
 
 Launch::Launch(ncm_ctx* ctx, KernelId id, cudaStream_t stream) : ctx_(ctx), id_(id), stream_(stream) {
   ProfState& p = ctx->prof;

@@ -28,6 +28,8 @@ enum KernelId {
   KID_DECODER_ELEMENTWISE,
   KID_CONV,
   KID_UPSAMPLE,
+  KID_KV_CACHE,
+  KID_LOGITS,
   KID_COUNT
 };
 extern const char* const kKernelNames[KID_COUNT];
@@ -149,6 +151,43 @@ class DeviceFlags {
  private:
   std::atomic<unsigned long long> bits_{0};
 };
+
+// Makes a context's device current for one entry point and puts the calling
+// thread's device back when it returns.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(const ncm_ctx* ctx) {
+    if (ctx == nullptr) {
+      status_ = ncm_fail(NCM_EINVAL, "null context");
+      return;
+    }
+    cudaError_t e = cudaGetDevice(&before_);
+    if (e == cudaSuccess && before_ != ctx->device) {
+      e = cudaSetDevice(ctx->device);
+      moved_ = e == cudaSuccess;
+    }
+    if (e != cudaSuccess) status_ = ncm_set_cuda_error(e);
+  }
+  ~DeviceGuard() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+  int status() const { return status_; }
+
+ private:
+  int before_ = 0;
+  bool moved_ = false;
+  int status_ = NCM_OK;
+};
+
+inline bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Whether [a, a + an) and [b, b + bn) (bytes) share any.
+inline bool ranges_overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + bn && y < x + an;
+}
 
 // Ensures the workspace holds at least `bytes`; returns its base or nullptr.
 void* ctx_workspace(ncm_ctx* ctx, size_t bytes);

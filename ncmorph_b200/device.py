@@ -62,6 +62,39 @@ def need(t: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple | None = N
     return t
 
 
+def need_rows(t: torch.Tensor, dtype: torch.dtype, name: str, device: torch.device, width: int) -> int:
+    """Validates a [rows, >= width] matrix whose rows may be strided (a column
+    slice of a wider matrix, say) and returns its row stride in elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.dim() != 2 or t.shape[1] < width:
+        raise ValueError(f"{name} must be a matrix of at least {width} columns, got {tuple(t.shape)}")
+    rows, stride = t.shape[0], t.stride(0)
+    if t.stride(1) != 1 or (rows > 1 and stride < t.shape[1]):
+        raise ValueError(f"{name} must have contiguous, separate rows")
+    # (a single row's stride says nothing: the row itself covers what is read)
+    return stride if rows > 1 else max(stride, t.shape[1] + 7 & ~7)
+
+
+def need_vec(t: torch.Tensor | None, dtype: torch.dtype, name: str, device: torch.device, n: int | None = None):
+    """Address of a contiguous vector argument (0 for None), validated."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be a contiguous vector{'' if n is None else f' of {n}'}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
 def sync(device: int | torch.device | None = None) -> None:
     """Waits for torch's current stream and reports device-side failures."""
     dev = torch.device("cuda", device) if isinstance(device, int) else (device or torch.device("cuda"))

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .device import context, need, ptr, stream_of
+from .device import context, need, need_rows, need_vec, ptr, stream_of
 
 MASK_MODES = {"causal": 0, "block_diagonal": 1, "block_causal": 2}
 bf16 = torch.bfloat16
@@ -64,6 +64,38 @@ def rope_tables(head_dim: int, theta: float, positions, llama3: tuple | None = N
         _lib.call("ncm_rope_tables_llama3_host", head_dim, float(theta), float(factor), float(low), float(high),
                   int(orig), vp(pos.ctypes.data), T, vp(c.ctypes.data), vp(s.ctypes.data))
     return c, s
+
+
+def rope_bf16(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int, head_dim: int,
+              interleaved: bool = False, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of the first `heads` heads of each row of x [T, >= heads *
+    head_dim] bf16 (rows may be strided, e.g. fused QKV rows), row t at position
+    positions[t] (int32) of the tables cos/sin [P, rotary_dim] f32 (rope_tables
+    for positions 0..P-1). rotary_dim columns of every head are rotated, as
+    halves (i, i + rotary_dim / 2) or, interleaved, as neighbours (2i, 2i + 1);
+    the others are copied. Rounded once to bf16. `inverse` rotates back: the
+    gradient. `out`: where to write (x itself: in place), default a new
+    [T, heads * head_dim]."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    dev = x.device
+    width = heads * head_dim
+    stride = need_rows(x, bf16, "x", dev, width)
+    T = x.shape[0]
+    P, rotary = cos.shape
+    need(cos, torch.float32, "cos")
+    need(sin, torch.float32, "sin", (P, rotary))
+    if cos.device != dev or sin.device != dev:
+        raise ValueError(f"cos and sin must be on {dev}")
+    pos = need_vec(positions, torch.int32, "positions", dev, T)
+    if out is None:
+        out = torch.empty((T, width), dtype=bf16, device=dev)
+    out_stride = need_rows(out, bf16, "out", dev, width)
+    if out.shape[0] != T:
+        raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
+    _lib.call("ncm_rope_bf16", context(dev), x.data_ptr(), stride, out.data_ptr(), out_stride, pos, cos.data_ptr(),
+              sin.data_ptr(), P, T, heads, head_dim, rotary, int(interleaved), int(inverse), stream_of(x))
+    return out
 
 
 def rms_norm_bf16(x: torch.Tensor, weight: torch.Tensor, eps: float, bias: torch.Tensor | None = None):
@@ -251,3 +283,66 @@ def tied_head_argmax(z: torch.Tensor, codebook: torch.Tensor, log_inv_T: float =
     _lib.call("ncm_tied_head_argmax", context(z.device), ptr(z), ptr(codebook), ptr(esq), ptr(bias),
               float(log_inv_T), ptr(codes), T, d, K, stream_of(z))
     return codes
+
+
+def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, token_start: torch.Tensor | None = None,
+                   prompt_lens: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                   frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   bias_start: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                   allowed_rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases and grammar masks on next-token logits [R, V] (f32 or
+    bf16, rows may be strided), as ncm_logits_process documents them; returns
+    f32 [R, V], or writes to `out` (f32, or bf16 for bf16 logits; logits itself:
+    in place). Row r's history is tokens[token_start[r] : token_start[r + 1]]
+    (int32), the first prompt_lens[r] of it its prompt. repetition, frequency,
+    presence [R] f32. Biases are bias[bias_start[r] : bias_start[r + 1]] of the
+    tokens bias_ids. allowed [M, ceil(V / 32)] int32 holds bit masks (bit v % 32
+    of word v / 32: token v may follow); row r uses mask allowed_rows[r] (int32,
+    -1: none), or mask r."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    if logits.dtype not in (torch.float32, bf16):
+        raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    dev = logits.device
+    R, V = logits.shape
+    stride = need_rows(logits, logits.dtype, "logits", dev, V)
+    if out is None:
+        out = torch.empty((R, V), dtype=torch.float32, device=dev)
+    if not isinstance(out, torch.Tensor) or out.dtype not in (torch.float32, logits.dtype):
+        raise TypeError(f"out must be a float32 or {logits.dtype} tensor")
+    out_stride = need_rows(out, out.dtype, "out", dev, V)
+    if tuple(out.shape) != (R, V):
+        raise ValueError(f"out must have shape {(R, V)}, got {tuple(out.shape)}")
+    i32, f32 = torch.int32, torch.float32
+    r = _lib.LogitRules()
+    if tokens is not None:
+        r.tokens = need_vec(tokens, i32, "tokens", dev)
+        r.num_tokens = tokens.shape[0]
+        r.token_start = need_vec(token_start, i32, "token_start", dev, R + 1)
+        r.prompt_lens = need_vec(prompt_lens, i32, "prompt_lens", dev, R)
+    elif prompt_lens is not None or token_start is not None:
+        raise ValueError("token_start and prompt_lens need tokens")
+    r.repetition = need_vec(repetition, f32, "repetition", dev, R)
+    r.frequency = need_vec(frequency, f32, "frequency", dev, R)
+    r.presence = need_vec(presence, f32, "presence", dev, R)
+    if bias is not None:
+        r.bias = need_vec(bias, f32, "bias", dev)
+        r.num_bias = bias.shape[0]
+        r.bias_ids = need_vec(bias_ids, i32, "bias_ids", dev, bias.shape[0])
+        r.bias_start = need_vec(bias_start, i32, "bias_start", dev, R + 1)
+    elif bias_ids is not None or bias_start is not None:
+        raise ValueError("bias_ids and bias_start need bias")
+    if allowed is not None:
+        r.allowed_stride = need_rows(allowed, i32, "allowed", dev, (V + 31) // 32)
+        r.allowed = allowed.data_ptr()
+        r.allowed_count = allowed.shape[0]
+        r.allowed_rows = need_vec(allowed_rows, i32, "allowed_rows", dev, R)
+    elif allowed_rows is not None:
+        raise ValueError("allowed_rows needs allowed")
+    types = {f32: 2, bf16: 0}
+    _lib.call("ncm_logits_process", context(dev), logits.data_ptr(), types[logits.dtype], stride, out.data_ptr(),
+              types[out.dtype], out_stride, R, V, ctypes.byref(r), stream_of(logits))
+    return out
