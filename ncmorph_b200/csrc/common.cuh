@@ -42,6 +42,16 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
 }
 
+#ifdef __CUDACC__
+// Two values to bf16 by the hardware's nearest-even conversion: f32_to_bf16 for
+// every value that is not NaN (a NaN becomes a NaN of other bits).
+__device__ __forceinline__ uint32_t pack_rn_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+#endif
+
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 }  // namespace ncm

@@ -4,11 +4,13 @@
 // A head's row of one token (head_dim bf16 values) belongs to head_dim / 8
 // neighbouring lanes, eight values each. Written, per row with A = max |x|:
 //   code = round(M x / A), scale = A / M, M = 127 (int8) or 448 (e4m3).
-// M x is exact in f32 (bf16 has 8 significant bits, M at most 7) and the
-// quotient is correctly rounded. A quotient that is not halfway between two
-// codes is off from halfway by at least 2^-17 of a code at the top of the
-// range (its numerator and A are integers of at most 15 and 8 bits), which is
-// more than its rounding error of 2^-18, so the codes are those of exact arithmetic.
+// A quotient M x / A that is not halfway between two codes is off from halfway
+// by 2^-16 or more, relative to itself: M x and A have at most 15 and 8
+// significant bits, so their nonzero differences from a halfway point are
+// whole units of at most 16 bits (13 for e4m3, whose halfway points have 5 bits).
+// x * fl(M / A) is off by 2^-23 at most. Rounded to 18 bits (Veltkamp's splitting) it is
+// halfway exactly where the quotient is, so the codes are those of exact
+// arithmetic, ties included, without a division per value.
 //
 // Bound: memory; no value is used twice.
 #include <algorithm>
@@ -19,6 +21,7 @@ namespace ncm {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kRowTokens = 32;  // rows that a block moves at most
 
 __device__ __forceinline__ uint16_t pack_e4m3x2(float lo, float hi) {
   uint16_t r;
@@ -40,43 +43,54 @@ __device__ __forceinline__ float2 f16x2_to_f32(uint32_t v) {
   return r;
 }
 
-// Eight values of a row -> its eight codes and the row's scale. LPR lanes hold the row.
-template <int FMT, int LPR>
-__device__ __forceinline__ uint2 quantise8(const uint4& v, float* scale) {
-  const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-  uint32_t top = 0;  // the largest magnitude, as bf16 bits (they order as integers)
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(e[i] & 0x7FFFu, (e[i] >> 16) & 0x7FFFu));
+// The largest magnitude of a row held by LPR lanes, as bf16 bits (they order as integers).
+template <int LPR>
+__device__ __forceinline__ uint32_t row_top(uint32_t top) {
 #pragma unroll
   for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top;
+}
+__device__ __forceinline__ uint32_t top_of(const uint4& v) {
+  const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(e[i] & 0x7FFFu, (e[i] >> 16) & 0x7FFFu));
+  return top;
+}
+
+// M / A for a row whose largest magnitude is `top`, and the power of two that
+// its values are multiplied by first (so that neither over- nor underflows).
+template <int FMT>
+__device__ __forceinline__ float code_factor(uint32_t top, float* pre) {
   constexpr float M = FMT == NCM_KV_INT8 ? 127.f : 448.f;
-  if (top >= 0x7F80u) {
-    *scale = __uint_as_float(0x7FC00000u);
-    return make_uint2(0u, 0u);
-  }
-  if (top == 0) {
-    *scale = 1.f;
-    return make_uint2(0u, 0u);
-  }
-  float big = __uint_as_float(top << 16);
-  *scale = __fdiv_rn(big, M);
-  // M x must not overflow: rows this large are brought down by a power of two first
-  const float f = top >= 0x7000u ? 0x1p-32f : 1.f;
-  big *= f;
+  *pre = top < 0x1000u ? 0x1p64f : 1.f;
+  if (top >= 0x7F80u || top == 0u) return 0.f;
+  return __fdiv_rn(M, __uint_as_float(top << 16) * *pre);
+}
+
+// Eight values of a row -> their codes. zero: a row without finite largest magnitude.
+template <int FMT>
+__device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top) {
+  float pre;
+  const float factor = code_factor<FMT>(top, &pre);
+  if (factor == 0.f) return make_uint2(0u, 0u);
+  const uint32_t e[4] = {v.x, v.y, v.z, v.w};
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    y[2 * i] = __fdiv_rn(bf16lo(e[i]) * f * M, big);
-    y[2 * i + 1] = __fdiv_rn(bf16hi(e[i]) * f * M, big);
+  for (int i = 0; i < 8; ++i) {
+    const float x = (i & 1) ? bf16hi(e[i >> 1]) : bf16lo(e[i >> 1]);
+    const float q = __fmul_rn(__fmul_rn(x, pre), factor);
+    const float c = __fmul_rn(q, 65.f);
+    y[i] = __fsub_rn(c, __fsub_rn(c, q));  // q rounded to 18 bits
   }
   uint32_t out[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if constexpr (FMT == NCM_KV_INT8) {
-      uint32_t w = 0;
+      uint32_t b[4];  // 1.5 * 2^23 + y rounds y to a whole number, ties to even; its low byte is the code
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w |= (static_cast<uint32_t>(__float2int_rn(y[4 * h + i])) & 0xFFu) << (8 * i);
-      out[h] = w;
+      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(y[4 * h + i], 12582912.f));
+      out[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     } else {
       out[h] = pack_e4m3x2(y[4 * h], y[4 * h + 1]) | (static_cast<uint32_t>(pack_e4m3x2(y[4 * h + 2], y[4 * h + 3])) << 16);
     }
@@ -85,14 +99,21 @@ __device__ __forceinline__ uint2 quantise8(const uint4& v, float* scale) {
 }
 
 template <int FMT>
-__device__ __forceinline__ uint4 dequantise8(const uint2& c, float scale) {
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  if (top >= 0x7F80u) return __uint_as_float(0x7FC00000u);
+  return top == 0u ? 1.f : __fdiv_rn(__uint_as_float(top << 16), FMT == NCM_KV_INT8 ? 127.f : 448.f);
+}
+
+template <int FMT>
+__device__ __forceinline__ uint4 dequantise8(uint32_t lo, uint32_t hi, float scale) {
   float y[8];
-  const uint32_t w[2] = {c.x, c.y};
+  const uint32_t w[2] = {lo, hi};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if constexpr (FMT == NCM_KV_INT8) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[4 * h + i] = static_cast<float>(static_cast<int8_t>(w[h] >> (8 * i)));
+      for (int i = 0; i < 4; ++i)  // 2^23 + 128 + code, less 2^23 + 128
+        y[4 * h + i] = __uint_as_float(__byte_perm(w[h] ^ 0x80808080u, 0x4B000000u, 0x7440 | i)) - 8388736.f;
     } else {
       const float2 a = f16x2_to_f32(e4m3x2_to_f16x2(static_cast<uint16_t>(w[h])));
       const float2 b = f16x2_to_f32(e4m3x2_to_f16x2(static_cast<uint16_t>(w[h] >> 16)));
@@ -102,8 +123,8 @@ __device__ __forceinline__ uint4 dequantise8(const uint2& c, float scale) {
       y[4 * h + 3] = b.y;
     }
   }
-  return make_uint4(pack_bf16x2(y[0] * scale, y[1] * scale), pack_bf16x2(y[2] * scale, y[3] * scale),
-                    pack_bf16x2(y[4] * scale, y[5] * scale), pack_bf16x2(y[6] * scale, y[7] * scale));
+  return make_uint4(pack_rn_bf16x2(y[0] * scale, y[1] * scale), pack_rn_bf16x2(y[2] * scale, y[3] * scale),
+                    pack_rn_bf16x2(y[4] * scale, y[5] * scale), pack_rn_bf16x2(y[6] * scale, y[7] * scale));
 }
 
 struct RowsArgs {
@@ -113,25 +134,18 @@ struct RowsArgs {
   uint16_t* k;           // the caller's rows (append only reads them)
   uint16_t* v;
   long long k_stride, v_stride;
-  int parts;        // warp-wide steps of one token's rows (its key heads, then its value heads)
-  int token_warps;  // warps that share one token
+  int tokens;     // rows of one block, at most kRowTokens
+  int part_rows;  // head rows that a block's threads hold at a time
   int* err;
 };
 
-// One warp per (token, share of its parts). In a step the warp's 32 lanes move
-// 32 / LPR head rows.
-template <int FMT, int HD, bool APPEND>
-__global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  constexpr int LPR = HD / 8, RPS = 32 / LPR, EB = FMT == NCM_KV_BF16 ? 2 : 1;
-  const int lane = threadIdx.x & 31;
-  const long long warp = static_cast<long long>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
-  const long long t = warp / a.token_warps;
-  const int share = static_cast<int>(warp - t * a.token_warps);
-  if (t >= a.batch.rows) return;
+// Slot of packed row t (page * page_size + offset), or -1 where there is none:
+// behind the last sequence, or in a sequence or page that does not fit, which is reported.
+template <bool APPEND>
+__device__ __forceinline__ int slot_of_row(const RowsArgs& a, long long t) {
+  if (t >= a.batch.rows) return -1;
   const int b = sequence_of_row(a.batch.token_start, a.batch.batch, t);
-  if (b < 0) return;
+  if (b < 0) return -1;
   const int first = __ldg(a.batch.token_start + b), n = __ldg(a.batch.token_start + b + 1) - first;
   int begin;
   if (APPEND) {
@@ -144,56 +158,92 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
   // a sequence that does not fit is skipped as a whole
   if (first < 0 || begin < 0 || static_cast<long long>(begin) + n > cap ||
       static_cast<long long>(first) + n > a.batch.rows) {
-    if (lane == 0) atomicOr(a.err, kErrBadIndex);
-    return;
+    atomicOr(a.err, kErrBadIndex);
+    return -1;
   }
   const int pos = begin + static_cast<int>(t - first);
   const int page = __ldg(a.batch.page_table + b * a.batch.table_stride + (pos >> a.pools.page_shift));
   if (page < 0 || page >= a.pools.num_pages) {
-    if (lane == 0) atomicOr(a.err, kErrBadIndex);
-    return;
+    atomicOr(a.err, kErrBadIndex);
+    return -1;
   }
-  const int off = pos & ((1 << a.pools.page_shift) - 1);
-  const int piece = lane % LPR;
-#pragma unroll 4
-  for (int p = share; p < a.parts; p += a.token_warps) {
-    const int r = p * RPS + lane / LPR;
-    const bool live = r < 2 * a.pools.kv_heads;
-    const bool is_v = r >= a.pools.kv_heads;
-    const int h = is_v ? r - a.pools.kv_heads : r;
-    uint16_t* row = (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + h * HD + piece * 8;
-    const long long slot = kv_slot(a.pools, page, h, off);
-    uint8_t* code = static_cast<uint8_t*>(is_v ? a.pools.v : a.pools.k) + (slot * HD + piece * 8) * EB;
-    float* scales = is_v ? a.pools.v_scale : a.pools.k_scale;
-    if constexpr (APPEND) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (live) x = *reinterpret_cast<const uint4*>(row);
-      if constexpr (FMT == NCM_KV_BF16) {
-        if (live) *reinterpret_cast<uint4*>(code) = x;
+  return (page << a.pools.page_shift) + (pos & ((1 << a.pools.page_shift) - 1));
+}
+
+// A block resolves its rows' slots (one lane each) and then moves them. A
+// thread keeps its eight values of a row (a head of the keys or the values:
+// blockIdx.y picks the part of the row) and walks over the block's rows, BATCH of
+// them loaded before the first is stored.
+template <int FMT, int HD, bool APPEND>
+__global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) {
+  __shared__ int slots[kRowTokens];
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr bool CODES = FMT != NCM_KV_BF16;
+  constexpr int LPR = HD / 8, EB = CODES ? 1 : 2, BATCH = 4;
+  const long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
+  for (int i = threadIdx.x; i < a.tokens; i += kRowThreads) slots[i] = slot_of_row<APPEND>(a, t0 + i);
+  __syncthreads();
+  const int lane_row = threadIdx.x / LPR, piece = threadIdx.x % LPR;
+  const int e = blockIdx.y * a.part_rows + lane_row % a.part_rows;  // head row: keys, then values
+  const int first = lane_row / a.part_rows, step = (kRowThreads / LPR) / a.part_rows;  // this thread's tokens
+  const bool idle = e >= 2 * a.pools.kv_heads || first >= step;
+  const bool is_v = e >= a.pools.kv_heads;
+  const int h = is_v ? e - a.pools.kv_heads : e;
+  const long long stride = is_v ? a.v_stride : a.k_stride;
+  uint16_t* rows = (is_v ? a.v : a.k) + t0 * stride + h * HD + piece * 8;
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.pools.v : a.pools.k) + piece * 8 * EB;
+  float* scales = is_v ? a.pools.v_scale : a.pools.k_scale;
+  for (int i0 = 0; i0 < a.tokens; i0 += BATCH * step) {
+    uint4 x[BATCH];
+    float scale[BATCH];
+    long long at[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * step + first;
+      const int slot = !idle && i < a.tokens ? slots[i] : -1;
+      at[k] = slot < 0 ? -1 : kv_slot(a.pools, slot >> a.pools.page_shift, h, slot & ((1 << a.pools.page_shift) - 1));
+      x[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (at[k] < 0) continue;
+      if constexpr (APPEND) {
+        x[k] = *reinterpret_cast<const uint4*>(rows + i * stride);
+      } else if constexpr (CODES) {
+        const uint2 c = *reinterpret_cast<const uint2*>(codes + at[k] * HD);
+        x[k].x = c.x;
+        x[k].y = c.y;
+        scale[k] = scales[at[k]];
       } else {
-        float scale;
-        const uint2 c = quantise8<FMT, LPR>(x, &scale);
-        if (live) {
-          *reinterpret_cast<uint2*>(code) = c;
-          if (piece == 0) scales[slot] = scale;
-        }
+        x[k] = *reinterpret_cast<const uint4*>(codes + at[k] * (HD * EB));
       }
-    } else if (live) {
-      if constexpr (FMT == NCM_KV_BF16)
-        *reinterpret_cast<uint4*>(row) = *reinterpret_cast<const uint4*>(code);
-      else
-        *reinterpret_cast<uint4*>(row) = dequantise8<FMT>(*reinterpret_cast<const uint2*>(code), scales[slot]);
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      uint16_t* row = rows + (i0 + k * step + first) * stride;
+      if constexpr (APPEND && CODES) {
+        const uint32_t top = row_top<LPR>(top_of(x[k]));
+        if (at[k] >= 0) {
+          *reinterpret_cast<uint2*>(codes + at[k] * HD) = quantise8<FMT>(x[k], top);
+          if (piece == 0) scales[at[k]] = scale_of<FMT>(top);
+        }
+      } else if (at[k] >= 0) {
+        if constexpr (APPEND)
+          *reinterpret_cast<uint4*>(codes + at[k] * (HD * EB)) = x[k];
+        else if constexpr (CODES)
+          *reinterpret_cast<uint4*>(row) = dequantise8<FMT>(x[k].x, x[k].y, scale[k]);
+        else
+          *reinterpret_cast<uint4*>(row) = x[k];
+      }
     }
   }
 }
 
 template <bool APPEND>
 int launch_rows(ncm_ctx* ctx, const ncm_kv_cache_t* c, RowsArgs& a, cudaStream_t st) {
-  const int lpr = c->head_dim / 8;
-  a.parts = ceil_div(2 * c->kv_heads, 32 / lpr);
-  // Few tokens: a warp for each part, so that the call is one step long. Many:
-  // one warp a token, which looks its sequence and page up once.
-  a.token_warps = a.batch.rows * a.parts <= 8 * static_cast<long long>(ctx->num_sms) ? a.parts : 1;
+  // Few rows: a block each, so that they reach every SM. Many: up to kRowTokens a
+  // block, which looks their slots up together.
+  a.tokens = static_cast<int>(std::min<int64_t>(kRowTokens, std::max<int64_t>(1, a.batch.rows / (4 * ctx->num_sms))));
+  a.part_rows = std::min(2 * c->kv_heads, kRowThreads / (c->head_dim / 8));
+  const int parts = ceil_div(2 * c->kv_heads, a.part_rows);
   a.err = ctx->d_err;
   using Kernel = void (*)(const RowsArgs);
   static const Kernel table[3][2] = {
@@ -201,8 +251,8 @@ int launch_rows(ncm_ctx* ctx, const ncm_kv_cache_t* c, RowsArgs& a, cudaStream_t
       {kv_rows_kernel<NCM_KV_INT8, 64, APPEND>, kv_rows_kernel<NCM_KV_INT8, 128, APPEND>},
       {kv_rows_kernel<NCM_KV_E4M3, 64, APPEND>, kv_rows_kernel<NCM_KV_E4M3, 128, APPEND>}};
   Launch _launch(ctx, KID_KV_CACHE, st);
-  NCM_CUDA_TRY(launch_pdl(table[c->format][c->head_dim == 128], dim3(ceil_div(a.batch.rows * a.token_warps, kRowThreads / 32)),
-                          dim3(kRowThreads), 0, st, 1, a));
+  NCM_CUDA_TRY(launch_pdl(table[c->format][c->head_dim == 128], dim3(ceil_div(a.batch.rows, a.tokens), parts), dim3(kRowThreads), 0,
+                          st, 1, a));
   return NCM_OK;
 }
 

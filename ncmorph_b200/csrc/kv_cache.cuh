@@ -80,20 +80,18 @@ inline int kv_check_rows(const char* what, const char* name, const void* p, int6
 }
 
 // The sequence that owns packed row t: the b with token_start[b] <= t <
-// token_start[b + 1], or -1. Called by whole warps with one t; token_start is
-// searched 32 ways at a time. Bounds that do not ascend can only give a wrong
-// b in range, whose own bounds the caller checks.
+// token_start[b + 1], or -1. Bounds that do not ascend can only give a wrong b
+// in range, whose own bounds the caller checks.
 __device__ __forceinline__ int sequence_of_row(const int32_t* token_start, int batch, long long t) {
-  const int lane = threadIdx.x & 31;
   int lo = 0, n = batch;  // the answer is in [lo, lo + n)
   while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int at = lane * step;
-    const bool le = at < n && __ldg(token_start + lo + at) <= t;
-    const unsigned hit = __ballot_sync(0xffffffffu, le);
-    const int last = hit == 0 ? 0 : 31 - __clz(hit);
-    lo += last * step;
-    n = min(step, n - last * step);
+    const int half = n >> 1;
+    if (__ldg(token_start + lo + half) <= t) {
+      lo += half;
+      n -= half;
+    } else {
+      n = half;
+    }
   }
   if (batch < 1 || __ldg(token_start + lo) > t || __ldg(token_start + lo + 1) <= t) return -1;
   return lo;

@@ -1,11 +1,12 @@
 // Rules on next-token logits (ncm_logits_process): repetition, frequency and
 // presence penalties, biases and grammar masks, in one pass over the logits.
 //
-// A block owns a slice of one row's vocabulary. It counts the slice's tokens
-// of the row's history in shared memory (bit 31: seen in the prompt; the rest:
-// times produced; integer atomics, so the order does not matter), finds the
-// first of its bias entries for each token, and then streams the slice: read,
-// change, write. Everything is f32, in separate operations in the documented order.
+// A block owns a slice of one row's vocabulary, eight or sixteen tokens a thread. It
+// loads its logits into registers first, and while they arrive counts the
+// slice's tokens of the row's history in shared memory (bit 31: seen in the
+// prompt; the rest: times produced; integer atomics, so the order does not
+// matter) and finds the first of its bias entries for each token. Then it
+// changes and writes. Everything is f32, in separate operations in the documented order.
 //
 // Bound: memory, each logit read and written once. The history is read once
 // per slice (from L2 after the first).
@@ -17,8 +18,7 @@
 namespace ncm {
 namespace {
 
-constexpr int kLogitThreads = 512;
-constexpr int kSlice = 8192;  // tokens of a block: 32 KB of counts, 32 KB of bias entries
+constexpr int kMaxThreads = 512;
 constexpr uint32_t kInPrompt = 0x80000000u;
 constexpr uint32_t kNoEntry = 0xFFFFFFFFu;
 constexpr uint32_t kRepeated = 0x80000000u;  // more than one bias entry of this token
@@ -41,104 +41,179 @@ __device__ __forceinline__ void row_range(const int32_t* start, long long total,
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float load_logit(const T* p);
-template <>
-__device__ __forceinline__ float load_logit(const float* p) {
-  return *p;
+// Eight neighbouring logits from / to a row; `left` of them exist. VEC: the row is 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* p, int left, float (&x)[8]) {
+  if (VEC && left >= 8) {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : 0.f;
+  }
 }
-template <>
-__device__ __forceinline__ float load_logit(const uint16_t* p) {
-  return bf16_to_f32(*p);
+template <bool VEC>
+__device__ __forceinline__ void load8(const uint16_t* p, int left, float (&x)[8]) {
+  if (VEC && left >= 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf16lo(e[i]);
+      x[2 * i + 1] = bf16hi(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < left ? bf16_to_f32(p[i]) : 0.f;
+  }
 }
-__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = f32_to_bf16(v); }
+template <bool VEC>
+__device__ __forceinline__ void store8(float* p, int left, const float (&x)[8]) {
+  if (VEC && left >= 8) {
+    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+    *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = x[i];
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint16_t* p, int left, const float (&x)[8]) {
+  if (VEC && left >= 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_rn_bf16x2(x[0], x[1]), pack_rn_bf16x2(x[2], x[3]),
+                                              pack_rn_bf16x2(x[4], x[5]), pack_rn_bf16x2(x[6], x[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = static_cast<uint16_t>(pack_rn_bf16x2(x[i], 0.f));
+  }
+}
 
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitArgs a) {
-  extern __shared__ uint32_t sh[];
+// GROUPS of eight neighbouring tokens a thread.
+template <typename TI, typename TO, bool VEC, int GROUPS>
+__global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) {
+  extern __shared__ __align__(16) uint32_t sh[];
   pdl_wait();
   pdl_launch_dependents();
-  const int r = blockIdx.y;
-  const long long v0 = static_cast<long long>(blockIdx.x) * kSlice;
-  const int n = static_cast<int>(min(static_cast<long long>(kSlice), a.vocab - v0));
+  const int r = blockIdx.y, threads = blockDim.x, slice = threads * 8 * GROUPS;
+  const long long v0 = static_cast<long long>(blockIdx.x) * slice;
+  const int n = static_cast<int>(min(static_cast<long long>(slice), a.vocab - v0));
+  const TI* in = static_cast<const TI*>(a.in) + r * a.in_stride + v0;
+  TO* out = static_cast<TO*>(a.out) + r * a.out_stride + v0;
+  float x[GROUPS][8];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int i = (g * threads + threadIdx.x) * 8;
+    load8<VEC>(in + i, n - i, x[g]);
+  }
   const ncm_logit_rules_t& R = a.r;
   const bool history = R.tokens != nullptr, biased = R.bias != nullptr;
   uint32_t* count = sh;
-  uint32_t* entry = sh + (history ? kSlice : 0);
+  uint32_t* entry = sh + (history ? slice : 0);
   int t_lo = 0, t_hi = 0, b_lo = 0, b_hi = 0;
   if (history) {
     row_range(R.token_start, R.num_tokens, r, &t_lo, &t_hi, a.err);
-    for (int i = threadIdx.x; i < n; i += kLogitThreads) count[i] = 0;
+    for (int i = threadIdx.x; i < slice / 4; i += threads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   if (biased) {
     row_range(R.bias_start, R.num_bias, r, &b_lo, &b_hi, a.err);
-    for (int i = threadIdx.x; i < n; i += kLogitThreads) entry[i] = kNoEntry;
+    if (b_hi > b_lo)
+      for (int i = threadIdx.x; i < slice / 4; i += threads)
+        reinterpret_cast<uint4*>(entry)[i] = make_uint4(kNoEntry, kNoEntry, kNoEntry, kNoEntry);
   }
-  __syncthreads();
+  // (everything that is one load away is asked for before the first wait)
   const int prompt = history && R.prompt_lens != nullptr ? __ldg(R.prompt_lens + r) : 0;
-  for (int i = t_lo + threadIdx.x; i < t_hi; i += kLogitThreads) {
-    const int id = __ldg(R.tokens + i);
-    if (id < 0 || id >= a.vocab) {
-      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
-      continue;
-    }
-    const long long j = id - v0;
-    if (j < 0 || j >= n) continue;
-    if (i - t_lo < prompt)
-      atomicOr(count + j, kInPrompt);
-    else
-      atomicAdd(count + j, 1u);
-  }
-  // the first entry of each token, and whether there are more
-  for (int i = b_lo + threadIdx.x; i < b_hi; i += kLogitThreads) {
-    const int id = __ldg(R.bias_ids + i);
-    if (id < 0 || id >= a.vocab) {
-      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
-      continue;
-    }
-    const long long j = id - v0;
-    if (j >= 0 && j < n) atomicMin(entry + j, static_cast<uint32_t>(i - b_lo));
-  }
-  if (b_hi > b_lo) {
-    __syncthreads();
-    for (int i = b_lo + threadIdx.x; i < b_hi; i += kLogitThreads) {
-      const long long j = __ldg(R.bias_ids + i) - v0;
-      if (j >= 0 && j < n && (entry[j] & ~kRepeated) != static_cast<uint32_t>(i - b_lo)) atomicOr(entry + j, kRepeated);
-    }
-  }
-  __syncthreads();
-  const uint32_t* mask = nullptr;
-  if (R.allowed != nullptr) {
-    const int m = R.allowed_rows != nullptr ? __ldg(R.allowed_rows + r) : r;
-    if (m >= 0 && m < R.allowed_count)
-      mask = R.allowed + m * R.allowed_stride;
-    else if (m != -1 && threadIdx.x == 0)
-      atomicOr(a.err, kErrBadIndex);
-  }
   const float rep = R.repetition != nullptr ? __ldg(R.repetition + r) : 1.f;
   const float freq = R.frequency != nullptr ? __ldg(R.frequency + r) : 0.f;
   const float pres = R.presence != nullptr ? __ldg(R.presence + r) : 0.f;
-  const TI* in = static_cast<const TI*>(a.in) + r * a.in_stride + v0;
-  TO* out = static_cast<TO*>(a.out) + r * a.out_stride + v0;
-  for (int i = threadIdx.x; i < n; i += kLogitThreads) {
-    float x = load_logit(in + i);
-    const uint32_t c = history ? count[i] : 0u;
-    if (c != 0u) {
-      x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      const uint32_t made = c & ~kInPrompt;
-      if (made != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(made))), pres);
+  const uint32_t* mask = nullptr;
+  uint32_t bits[GROUPS];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) bits[g] = 0xFFu;
+  if (R.allowed != nullptr) {
+    const int m = R.allowed_rows != nullptr ? __ldg(R.allowed_rows + r) : r;
+    if (m >= 0 && m < R.allowed_count) {
+      mask = R.allowed + m * R.allowed_stride + (v0 >> 5);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const int i = (g * threads + threadIdx.x) * 8;
+        if (i < n) bits[g] = __ldg(mask + (i >> 5)) >> (i & 31);
+      }
+    } else if (m != -1 && threadIdx.x == 0) {
+      atomicOr(a.err, kErrBadIndex);
     }
-    const uint32_t e = biased ? entry[i] : kNoEntry;
-    if (e != kNoEntry) {
-      const int at = b_lo + static_cast<int>(e & ~kRepeated);
-      x = __fadd_rn(x, __ldg(R.bias + at));
-      if (e & kRepeated)
-        for (int k = at + 1; k < b_hi; ++k)
-          if (__ldg(R.bias_ids + k) == v0 + i) x = __fadd_rn(x, __ldg(R.bias + k));
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = t_lo + threadIdx.x; i < t_hi; i += threads) {
+    const int id = __ldg(R.tokens + i);
+    const long long j = id - v0;
+    if (id < 0 || id >= a.vocab) {
+      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
+    } else if (j >= 0 && j < n) {
+      if (i - t_lo < prompt)
+        atomicOr(count + j, kInPrompt);
+      else
+        atomicAdd(count + j, 1u);
     }
-    if (mask != nullptr && !((__ldg(mask + ((v0 + i) >> 5)) >> (i & 31)) & 1u)) x = -__uint_as_float(0x7F800000u);
-    store_logit(out + i, x);
+  }
+  // the first entry of each token, and whether there are more
+  for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
+    const int id = __ldg(R.bias_ids + i);
+    const long long j = id - v0;
+    if (id < 0 || id >= a.vocab) {
+      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
+    } else if (j >= 0 && j < n) {
+      atomicMin(entry + j, static_cast<uint32_t>(i - b_lo));
+    }
+  }
+  __syncthreads();
+  if (b_hi > b_lo) {
+    for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
+      const long long j = __ldg(R.bias_ids + i) - v0;
+      if (j >= 0 && j < n && (entry[j] & ~kRepeated) != static_cast<uint32_t>(i - b_lo)) atomicOr(entry + j, kRepeated);
+    }
+    __syncthreads();
+  }
+  const float inv = __frcp_rn(rep);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int i = (g * threads + threadIdx.x) * 8;
+    if (i >= n) continue;
+    if (history) {
+      uint32_t c[8];
+      *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(count + i);
+      *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(count + i + 4);
+      if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // l / rep as l * (1 / rep): within an f32 rounding, a third of the instructions
+          float y = __fmul_rn(x[g][e], x[g][e] > 0.f ? inv : rep);
+          const uint32_t made = c[e] & ~kInPrompt;
+          if (made != 0u) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(made))), pres);
+          if (c[e] != 0u) x[g][e] = y;
+        }
+      }
+    }
+    if (b_hi > b_lo) {
+      uint32_t c[8];
+      *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(entry + i);
+      *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(entry + i + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (c[e] == kNoEntry) continue;
+        const int at = b_lo + static_cast<int>(c[e] & ~kRepeated);
+        x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + at));
+        if (c[e] & kRepeated)
+          for (int k = at + 1; k < b_hi; ++k)
+            if (__ldg(R.bias_ids + k) == v0 + i + e) x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + k));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (!((bits[g] >> e) & 1u)) x[g][e] = -__uint_as_float(0x7F800000u);
+    store8<VEC>(out + i, n - i, x[g]);
   }
 }
 
@@ -183,18 +258,35 @@ extern "C" int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dt
   if (!in_place && ranges_overlap(logits, isz * ((rows - 1) * stride + vocab), out, osz * ((rows - 1) * out_stride + vocab)))
     return ncm_fail(NCM_EINVAL, "logits_process: logits and out overlap without being the same rows");
   LogitArgs a{logits, out, stride, out_stride, vocab, r, ctx->d_err};
-  const size_t smem = sizeof(uint32_t) * kSlice * ((r.tokens != nullptr) + (r.bias != nullptr));
-  auto kernel = dtype == NCM_DTYPE_F32      ? logits_kernel<float, float>
-                : out_dtype == NCM_DTYPE_F32 ? logits_kernel<uint16_t, float>
-                                             : logits_kernel<uint16_t, uint16_t>;
-  static DeviceFlags ready[3];
-  DeviceFlags& flag = ready[dtype == NCM_DTYPE_F32 ? 0 : out_dtype == NCM_DTYPE_F32 ? 1 : 2];
+  // The longest slice (its history is read the fewest times) that still gives
+  // every SM four blocks; where that is not to be had, short slices of eight tokens a
+  // thread, so that more threads read the history.
+  int threads = kMaxThreads, groups = 2;
+  while (threads > 128 && rows * ceil_div(vocab, threads * 8 * groups) < 4 * ctx->num_sms) {
+    groups = 1;
+    threads /= 2;
+  }
+  const int slice = threads * 8 * groups;
+  const size_t smem = sizeof(uint32_t) * slice * ((r.tokens != nullptr) + (r.bias != nullptr));
+  const bool vec = aligned_to(logits, 16) && aligned_to(out, 16) && stride * isz % 16 == 0 && out_stride * osz % 16 == 0;
+  using Kernel = void (*)(const LogitArgs);
+  static const Kernel table[3][2][2] = {
+      {{logits_kernel<float, float, false, 1>, logits_kernel<float, float, false, 2>},
+       {logits_kernel<float, float, true, 1>, logits_kernel<float, float, true, 2>}},
+      {{logits_kernel<uint16_t, float, false, 1>, logits_kernel<uint16_t, float, false, 2>},
+       {logits_kernel<uint16_t, float, true, 1>, logits_kernel<uint16_t, float, true, 2>}},
+      {{logits_kernel<uint16_t, uint16_t, false, 1>, logits_kernel<uint16_t, uint16_t, false, 2>},
+       {logits_kernel<uint16_t, uint16_t, true, 1>, logits_kernel<uint16_t, uint16_t, true, 2>}}};
+  const int kind = dtype == NCM_DTYPE_F32 ? 0 : out_dtype == NCM_DTYPE_F32 ? 1 : 2;
+  const Kernel kernel = table[kind][vec][groups - 1];
+  static DeviceFlags ready[3][2][2];
+  DeviceFlags& flag = ready[kind][vec][groups - 1];
   if (!flag.test(ctx->device)) {
-    NCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kSlice));
+    NCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * sizeof(uint32_t) * kMaxThreads * 16));
     flag.set(ctx->device);
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Launch _launch(ctx, KID_LOGITS, st);
-  NCM_CUDA_TRY(launch_pdl(kernel, dim3(ceil_div(vocab, kSlice), static_cast<unsigned>(rows)), dim3(kLogitThreads), smem, st, 1, a));
+  NCM_CUDA_TRY(launch_pdl(kernel, dim3(ceil_div(vocab, slice), static_cast<unsigned>(rows)), dim3(threads), smem, st, 1, a));
   return NCM_OK;
 }

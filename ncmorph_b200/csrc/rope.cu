@@ -27,14 +27,9 @@ struct RopeArgs {
   int rot_units, head_units;  // units of one head: rotated ones, and all
   int row_units;              // heads * head_units
   int tokens;                 // tokens of one block
-  uint32_t magic_row, magic_head;
-  float sign;  // -1 for the inverse rotation
+  float sign;                 // -1 for the inverse rotation
   int* err;
 };
-
-constexpr int kRopeThreads = 256;
-
-__device__ __forceinline__ uint4 load16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   const float ra = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
@@ -42,73 +37,107 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   a = ra;
 }
 
-// A unit is what one thread moves at a time. VEC: 16-byte pieces (half layout:
+// A unit is what one thread moves at a time: VEC: 16-byte pieces (half layout:
 // the two pieces of eight pairs; interleaved: one piece of four pairs; behind
-// the rotated columns: one piece copied); otherwise one pair, or one column copied.
+// the rotated columns: one piece copied); otherwise one pair, or one column
+// copied. A thread keeps its unit (blockIdx.y picks the part of the row) and
+// walks over the block's tokens, BATCH of them loaded before the first is used.
 template <bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
   pdl_wait();
   pdl_launch_dependents();
+  constexpr int BATCH = 4;
+  constexpr bool TWO = !INTERLEAVED || !VEC;  // a unit is two loads
+  constexpr int PAIRS = VEC ? (INTERLEAVED ? 4 : 8) : 1;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x;
+  if (u >= a.row_units) return;
+  const int head = u / a.head_units, w = u - head * a.head_units;
+  const bool rot = w < a.rot_units;
+  int i = head * a.head_dim, step = 0;  // the unit's column, and how far its second load is
+  if (rot) {
+    i += VEC ? 8 * w : INTERLEAVED ? 2 * w : w;
+    step = VEC || !INTERLEAVED ? a.half : 1;
+  } else {
+    i += a.rotary + (VEC ? 8 : 1) * (w - a.rot_units);
+  }
   const long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
-  const int n = static_cast<int>(min(static_cast<long long>(a.tokens), a.T - t0)) * a.row_units;
-#pragma unroll 2
-  for (int u = threadIdx.x; u < n; u += kRopeThreads) {
-    const int tl = a.tokens == 1 ? 0 : a.row_units == 1 ? u : static_cast<int>(__umulhi(u, a.magic_row));
-    const int ur = u - tl * a.row_units;
-    const int head = a.head_units == 1 ? ur : static_cast<int>(__umulhi(ur, a.magic_head));
-    const int w = ur - head * a.head_units;
-    const long long t = t0 + tl;
-    const int pos = __ldg(a.positions + t);
-    if (pos < 0 || pos >= a.table_rows) {
-      if (ur == 0) atomicOr(a.err, kErrBadIndex);
-      continue;
-    }
-    const uint16_t* xr = a.x + t * a.x_stride + static_cast<long long>(head) * a.head_dim;
-    uint16_t* yr = a.y + t * a.y_stride + static_cast<long long>(head) * a.head_dim;
-    const float* cr = a.cos_t + static_cast<long long>(pos) * a.rotary;
-    const float* sr = a.sin_t + static_cast<long long>(pos) * a.rotary;
-    if (w >= a.rot_units) {
+  const int n = static_cast<int>(min(static_cast<long long>(a.tokens), a.T - t0));
+  const uint16_t* src = a.x + t0 * a.x_stride + i;
+  uint16_t* dst = a.y + t0 * a.y_stride + i;
+  for (int k0 = 0; k0 < n; k0 += BATCH) {
+    uint4 v[BATCH], z[BATCH];
+    int pos[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (k0 + k >= n) break;
+      const uint16_t* p = src + k * a.x_stride;
       if constexpr (VEC) {
-        const int i = a.rotary + (w - a.rot_units) * 8;
-        *reinterpret_cast<uint4*>(yr + i) = load16(xr + i);
+        v[k] = *reinterpret_cast<const uint4*>(p);
+        if (TWO && rot) z[k] = *reinterpret_cast<const uint4*>(p + step);
       } else {
-        const int i = a.rotary + (w - a.rot_units);
-        yr[i] = xr[i];
+        v[k].x = *p;
+        if (rot) z[k].x = p[step];
       }
-    } else if constexpr (!VEC) {
-      const int i = INTERLEAVED ? 2 * w : w, j = INTERLEAVED ? 2 * w + 1 : w + a.half;
-      float p = bf16_to_f32(xr[i]), q = bf16_to_f32(xr[j]);
-      rotate(p, q, cr[w], a.sign * sr[w]);
-      yr[i] = f32_to_bf16(p);
-      yr[j] = f32_to_bf16(q);
-    } else if constexpr (INTERLEAVED) {
-      const uint4 v = load16(xr + 8 * w);
-      uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float p = bf16lo(e[k]), q = bf16hi(e[k]);
-        rotate(p, q, cr[4 * w + k], a.sign * sr[4 * w + k]);
-        e[k] = pack_bf16x2(p, q);
-      }
-      *reinterpret_cast<uint4*>(yr + 8 * w) = make_uint4(e[0], e[1], e[2], e[3]);
-    } else {
-      const uint4 v = load16(xr + 8 * w), z = load16(xr + a.half + 8 * w);
-      uint32_t e[4] = {v.x, v.y, v.z, v.w}, f[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float p0 = bf16lo(e[k]), q0 = bf16lo(f[k]), p1 = bf16hi(e[k]), q1 = bf16hi(f[k]);
-        rotate(p0, q0, cr[8 * w + 2 * k], a.sign * sr[8 * w + 2 * k]);
-        rotate(p1, q1, cr[8 * w + 2 * k + 1], a.sign * sr[8 * w + 2 * k + 1]);
-        e[k] = pack_bf16x2(p0, p1);
-        f[k] = pack_bf16x2(q0, q1);
-      }
-      *reinterpret_cast<uint4*>(yr + 8 * w) = make_uint4(e[0], e[1], e[2], e[3]);
-      *reinterpret_cast<uint4*>(yr + a.half + 8 * w) = make_uint4(f[0], f[1], f[2], f[3]);
+      pos[k] = __ldg(a.positions + t0 + k0 + k);
     }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (k0 + k >= n) break;
+      uint16_t* q = dst + k * a.y_stride;
+      if (pos[k] < 0 || pos[k] >= a.table_rows) {
+        if (w == 0) atomicOr(a.err, kErrBadIndex);
+        continue;
+      }
+      if (rot) {
+        const long long at = static_cast<long long>(pos[k]) * a.rotary + PAIRS * w;
+        float c[PAIRS], s[PAIRS];
+        if constexpr (VEC) {
+#pragma unroll
+          for (int e = 0; e < PAIRS; e += 4) {
+            *reinterpret_cast<float4*>(&c[e]) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at + e));
+            *reinterpret_cast<float4*>(&s[e]) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at + e));
+          }
+        } else {
+          c[0] = __ldg(a.cos_t + at);
+          s[0] = __ldg(a.sin_t + at);
+        }
+        uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w}, f[4] = {z[k].x, z[k].y, z[k].z, z[k].w};
+        if constexpr (!VEC) {
+          float p0 = bf16lo(e[0]), q0 = bf16lo(f[0]);
+          rotate(p0, q0, c[0], a.sign * s[0]);
+          const uint32_t both = pack_rn_bf16x2(p0, q0);
+          v[k].x = both & 0xFFFFu;
+          q[step] = static_cast<uint16_t>(both >> 16);
+        } else if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float p0 = bf16lo(e[x]), q0 = bf16hi(e[x]);
+            rotate(p0, q0, c[x], a.sign * s[x]);
+            e[x] = pack_rn_bf16x2(p0, q0);
+          }
+          v[k] = make_uint4(e[0], e[1], e[2], e[3]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float p0 = bf16lo(e[x]), q0 = bf16lo(f[x]), p1 = bf16hi(e[x]), q1 = bf16hi(f[x]);
+            rotate(p0, q0, c[2 * x], a.sign * s[2 * x]);
+            rotate(p1, q1, c[2 * x + 1], a.sign * s[2 * x + 1]);
+            e[x] = pack_rn_bf16x2(p0, p1);
+            f[x] = pack_rn_bf16x2(q0, q1);
+          }
+          v[k] = make_uint4(e[0], e[1], e[2], e[3]);
+          *reinterpret_cast<uint4*>(q + step) = make_uint4(f[0], f[1], f[2], f[3]);
+        }
+      }
+      if constexpr (VEC)
+        *reinterpret_cast<uint4*>(q) = v[k];
+      else
+        *q = static_cast<uint16_t>(v[k].x);
+    }
+    src += BATCH * a.x_stride;
+    dst += BATCH * a.y_stride;
   }
 }
-
-uint32_t magic_of(int d) { return static_cast<uint32_t>((0x100000000ull + d - 1) / d); }
 
 }  // namespace
 }  // namespace ncm
@@ -153,19 +182,21 @@ extern "C" int ncm_rope_bf16(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride
   a.half = rotary_dim / 2;
   a.sign = inverse ? -1.f : 1.f;
   a.err = ctx->d_err;
-  const bool vec = aligned_to(x, 16) && aligned_to(y, 16) && x_stride % 8 == 0 && y_stride % 8 == 0 &&
+  const bool vec = aligned_to(x, 16) && aligned_to(y, 16) && aligned_to(cos_t, 16) && aligned_to(sin_t, 16) && x_stride % 8 == 0 && y_stride % 8 == 0 &&
                    head_dim % 8 == 0 && (interleaved ? rotary_dim : a.half) % 8 == 0;
   const int copied = in_place ? 0 : head_dim - rotary_dim;
   a.rot_units = vec ? (interleaved ? rotary_dim / 8 : a.half / 8) : a.half;
   a.head_units = a.rot_units + (vec ? copied / 8 : copied);
   a.row_units = heads * a.head_units;
-  a.tokens = std::max(1, 2 * kRopeThreads / a.row_units);
-  a.magic_row = magic_of(a.row_units);
-  a.magic_head = magic_of(a.head_units);
+  // Blocks of equal parts of a row. One token a block where there are few, so
+  // that they reach every SM; up to 8 where there are enough for four blocks an SM.
+  const int parts = ceil_div(a.row_units, 256);
+  const int threads = ceil_div(ceil_div(a.row_units, parts), 32) * 32;
+  a.tokens = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, T * parts / (4 * ctx->num_sms))));
   auto kernel = vec ? (interleaved ? rope_rows_kernel<true, true> : rope_rows_kernel<true, false>)
                     : (interleaved ? rope_rows_kernel<false, true> : rope_rows_kernel<false, false>);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Launch _launch(ctx, KID_DECODER_ELEMENTWISE, st);
-  NCM_CUDA_TRY(launch_pdl(kernel, dim3(ceil_div(T, a.tokens)), dim3(kRopeThreads), 0, st, 1, a));
+  NCM_CUDA_TRY(launch_pdl(kernel, dim3(ceil_div(T, a.tokens), parts), dim3(threads), 0, st, 1, a));
   return NCM_OK;
 }

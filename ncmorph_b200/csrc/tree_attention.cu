@@ -7,23 +7,33 @@
 // node) form tiles of up to ROWS rows; an item is (sequence, kv head, tile).
 // A CTA holds KG key groups of RG warps. A key group takes every KG-th tile of
 // 32 keys through a cp.async ring of its own (zero-filled behind the last
-// key), its warps each hold 16 MT query rows in registers: S = Q K^T and P V
-// are m16n8k16 products with f32 sums, P never leaves the registers, and codes
-// become bf16 in registers (both code types are exact in bf16; a key's scale
-// multiplies its score, a value's scale its probability). The maximum m is
-// only moved when a score passes it by 2^8, so most tiles neither reduce over
-// lanes nor rescale. The key groups' sums meet in shared memory at the end.
+// key); each of its warps holds 8 NT query rows in registers.
+//
+// Products are m16n8k16 with the keys on the 16-row side, S^T = K Q^T and
+// O^T = V^T P^T: a decoded token has few rows (4 for 32 query heads over 8), and
+// eight of them cost half of what sixteen would. S^T's registers become
+// P^T's by an 8x8 transposition in the warp (movmatrix). S sums over head_dim in any
+// order, so a lane reads 16 consecutive bytes of a key and Q's fragments are
+// permuted to match.
+//
+// Codes are used as they are: int8 and e4m3 values are exact in f16, a key's
+// scale multiplies its scores, and a value's scale s enters its probability's
+// exponent, p' = 2^(t + log2 s - m'), with a maximum m' of its own. P is then f16,
+// which costs 2^-12 of each term. Q is bf16 and becomes f16 with a power of two
+// of its row taken out; what is then below f16's range is 2^-30 of the
+// row's largest. A bf16 cache is multiplied in bf16 (its values do not fit f16's
+// range), with P rounded to bf16: 2^-9 of each term, about as much again as the output's
+// own rounding.
+//
+// A maximum is only moved when a score passes it by 2^8, so most tiles
+// neither reduce over lanes nor rescale.
 //
 // Split: items are cut into units of unit_keys keys, and every CTA of one wave
 // takes the same number of consecutive units, whatever the sequences' lengths
 // are (they are known on the device only). A CTA that ends inside an item
 // leaves its sums in the workspace: slot 2c for an item begun by an earlier
-// CTA, slot 2c + 1 for one that goes on in the next. merge_kernel adds the
+// CTA, slot 2c + 1 for one that goes on in the next. tree_merge_kernel adds the
 // slots of such items up, in order.
-//
-// Order of contractions: the m16n8k16 products sum over head_dim in any order,
-// so a lane reads 16 consecutive bytes of a key, and Q's fragments are
-// permuted to match (lane % 4 = c holds the same dims of Q and K).
 #include <algorithm>
 
 #include "kv_cache.cuh"
@@ -47,7 +57,7 @@ struct TreeArgs {
   uint16_t* out;
   long long out_stride;
   float* lse;
-  float* part;  // [2 * grid][ROWS][2 + HD]: maximum, sum, values
+  float* part;  // [2 * grid][ROWS][4 + HD]: m, sum of p, m', -, values
   int unit_keys;
   int grid;  // CTAs of the attention kernel
   int* err;
@@ -59,10 +69,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c += A B, m16n8k16; HALF: f16 operands, otherwise bf16.
+template <bool HALF>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
@@ -95,38 +118,40 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t pack_rn_f16x2(float lo, float hi) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// Bytes I and J of w as two bf16 values, exactly. int8: 128 + (low seven bits) minus
-// 128 or 256, by the sign bit. e4m3: the code's exponent and mantissa moved into
-// bf16's fields are the value times 2^-120 (subnormal codes included).
-template <int FMT, int I, int J>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+// Four codes as two pairs of f16, exactly: bytes (0, 1) and (2, 3).
+template <int FMT>
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t* lo, uint32_t* hi) {
   if constexpr (FMT == NCM_KV_INT8) {
-    const uint32_t x = prmt(w, 0x43u, 0x4040u | I | (J << 8));  // bytes: I, 0x43, J, 0x43
-    return sub_bf16x2(x & 0x437F437Fu, x & 0x43804380u);
+    w ^= 0x80808080u;  // 128 + code; 0x6400 | b is 1024 + b
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*lo) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*hi) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
   } else {
-    const uint32_t x = prmt(w, 0u, 0x0404u | (I << 4) | (J << 12));  // bytes: 0, I, 0, J
-    const uint32_t y = ((x & 0x7F007F00u) >> 4) | (x & 0x80008000u);
-    return mul_bf16x2(y, 0x7B807B80u);  // 2^120
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(*lo), "=r"(*hi)
+        : "r"(w));
   }
 }
-
-__device__ __forceinline__ uint32_t pack_rn(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
+// The same of bytes (0, 2) and (1, 3).
+template <int FMT>
+__device__ __forceinline__ void code_pairs_strided(uint32_t w, uint32_t* even, uint32_t* odd) {
+  if constexpr (FMT == NCM_KV_INT8) {
+    w ^= 0x80808080u;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*even) : "r"(__byte_perm(w, 0x64646464u, 0x4240)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*odd) : "r"(__byte_perm(w, 0x64646464u, 0x4341)), "r"(0x64806480u));
+  } else {
+    code_pairs<FMT>(__byte_perm(w, 0u, 0x3120), even, odd);
+  }
 }
 
 // What one sequence contributes: its nodes (0 where its numbers do not fit), keys and units.
@@ -210,10 +235,10 @@ __device__ __forceinline__ uint32_t mask_window(const uint32_t* row, int words, 
 }
 __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
-template <int HD, int FMT, int MT, int RG, int KG>
+template <int HD, int FMT, int NT, int RG, int KG>
 struct TreeShape {
   static constexpr int kThreads = 32 * RG * KG;
-  static constexpr int kRows = 16 * MT * RG;
+  static constexpr int kRows = 8 * NT * RG;
   static constexpr int kRowBytes = HD * (FMT == NCM_KV_BF16 ? 2 : 1);
   static constexpr int kStageBytes = 2 * kTile * kRowBytes + (FMT == NCM_KV_BF16 ? 0 : 2 * kTile * 4);
   // two tiles in flight beside the one in use
@@ -234,13 +259,24 @@ __device__ __forceinline__ uint32_t piece_at(int key, int chunk) {
     return key * RB + ((chunk ^ (((key & 1) << 2) | ((key >> 1) & 3))) << 4);
 }
 
-template <int HD, int FMT, int MT, int RG, int KG>
+// 2^(d / 2), twice: the values' sums are brought from their maximum to the
+// scores' by 2^d, which alone may pass f32's range.
+__device__ __forceinline__ float half_power(float d) { return ex2(0.5f * d); }
+// half_power(d) / sum; 0 for a row that saw nothing.
+__device__ __forceinline__ float out_factor(float sum, float d) { return sum == 0.f ? 0.f : __fdiv_rn(half_power(d), sum); }
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  return sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
+}
+
+template <int HD, int FMT, int NT, int RG, int KG>
 __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const TreeArgs a) {
-  using S = TreeShape<HD, FMT, MT, RG, KG>;
+  using S = TreeShape<HD, FMT, NT, RG, KG>;
+  constexpr bool CODES = FMT != NCM_KV_BF16;
   constexpr int RB = S::kRowBytes, CPR = RB / 16, ROWS = S::kRows, NST = S::kStages;
-  constexpr int KS = HD / 16;       // k-steps of S
-  constexpr int WPC = FMT == NCM_KV_BF16 ? 2 : 4;  // k-steps in a 16-byte piece
-  constexpr int DPC = FMT == NCM_KV_BF16 ? 8 : 16;  // dims in a 16-byte piece
+  constexpr int KS = HD / 16;               // k-steps of S
+  constexpr int WPC = CODES ? 4 : 2;        // k-steps in a 16-byte piece
+  constexpr int DPC = CODES ? 16 : 8;       // dims in a 16-byte piece
+  constexpr int DT = HD / 16;               // 16-dim tiles of O^T
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kg = warp / RG, rg = warp % RG;
@@ -266,8 +302,8 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
   };
 
   for (long long at = lo; at < hi && b < a.batch.batch;) {
-    Seq s = load_seq(a, b, false);
-    int units = units_of(a, s);
+    const Seq s = load_seq(a, b, false);
+    const int units = units_of(a, s);
     const int tiles = tiles_of<ROWS>(a, s);
     if (inside >= static_cast<long long>(units) * tiles * a.pools.kv_heads) {  // (empty sequences too)
       ++b;
@@ -281,48 +317,11 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
     const int key0 = u0 * a.unit_keys, key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) * a.unit_keys));
     const int live_rows = s.n * a.group - row0;  // rows of this tile that exist (may be more than ROWS)
 
-    // ---- this warp's query rows, in fragment order
-    uint32_t qf[MT][KS][4];
-    int node[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = rg * 16 * MT + mt * 16 + r + 8 * e;
-        const bool live = row < live_rows;
-        const int i = live ? (row0 + row) / a.group : 0;
-        const int head = kvh * a.group + (live ? (row0 + row) - i * a.group : 0);
-        node[mt][e] = live ? i : -1;
-        const uint16_t* src = a.q + (s.first + static_cast<long long>(i)) * a.q_stride + head * HD;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int d = ((ks / WPC) * 4 + c) * DPC + (ks % WPC) * 4;
-          uint2 v = make_uint2(0u, 0u);
-          if (live) v = *reinterpret_cast<const uint2*>(src + d);
-          qf[mt][ks][e] = v.x;
-          qf[mt][ks][2 + e] = v.y;
-        }
-      }
-
-    float o[MT][HD / 8][4];
-    float m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[mt][e] = kFirstMax;
-        l[mt][e] = 0.f;
-      }
-#pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
-    }
-
     // ---- this key group's tiles: key0 + 32 (kg + KG i)
     const int32_t* table = a.batch.page_table + b * a.batch.table_stride;
     const int ntiles = (key1 - key0 + kTile - 1) / kTile;
     const int mine = ntiles > kg ? (ntiles - kg + KG - 1) / KG : 0;
+    const int page_mask = (1 << a.pools.page_shift) - 1;
     // page of key (lane) of tile i, or -1
     auto page_of = [&](int i) {
       const int key = key0 + kTile * (kg + KG * i) + lane;
@@ -339,23 +338,37 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
         const int base = key0 + kTile * (kg + KG * i);
         const uint32_t st = ring + (i % NST) * S::kStageBytes;
         constexpr int PER = kTile * CPR / (32 * RG);
+        const int off = (base + lane) & page_mask;
+        const long long slot = pages >= 0 ? kv_slot(a.pools, pages, kvh, off) : 0;
+        if (a.pools.page_shift >= 5) {  // the tile is one run of its page
+          const long long first = __shfl_sync(0xffffffffu, slot, 0) * RB + gt * 16;
+          const int live = __popc(__ballot_sync(0xffffffffu, pages >= 0));  // its first keys
+          const uint8_t* ks = static_cast<const uint8_t*>(a.pools.k) + first;
+          const uint8_t* vs = static_cast<const uint8_t*>(a.pools.v) + first;
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-          const int idx = x * 32 * RG + gt;
-          const int key = idx / CPR, chunk = idx % CPR;
-          const int p = __shfl_sync(0xffffffffu, pages, key);
-          const bool live = p >= 0;
-          const long long slot = live ? kv_slot(a.pools, p, kvh, (base + key) & ((1 << a.pools.page_shift) - 1)) : 0;
-          const long long byte = slot * RB + chunk * 16;
-          cp16(st + piece_at<RB>(key, chunk), static_cast<const uint8_t*>(a.pools.k) + byte, live);
-          cp16(st + kTile * RB + piece_at<RB>(key, chunk), static_cast<const uint8_t*>(a.pools.v) + byte, live);
+          for (int x = 0; x < PER; ++x) {
+            const int idx = x * 32 * RG + gt;
+            const int key = idx / CPR;
+            const uint32_t to = st + piece_at<RB>(key, idx % CPR);
+            cp16(to, ks + (key < live ? x * 512 * RG : 0), key < live);
+            cp16(to + kTile * RB, vs + (key < live ? x * 512 * RG : 0), key < live);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < PER; ++x) {
+            const int idx = x * 32 * RG + gt;
+            const int key = idx / CPR, chunk = idx % CPR;
+            const bool live = __shfl_sync(0xffffffffu, pages, key) >= 0;
+            const long long byte = __shfl_sync(0xffffffffu, slot, key) * RB + chunk * 16;
+            const uint32_t to = st + piece_at<RB>(key, chunk);
+            cp16(to, static_cast<const uint8_t*>(a.pools.k) + byte, live);
+            cp16(to + kTile * RB, static_cast<const uint8_t*>(a.pools.v) + byte, live);
+          }
         }
-        if constexpr (FMT != NCM_KV_BF16) {
+        if constexpr (CODES) {
           if (rg == 0) {
-            const bool live = pages >= 0;
-            const long long slot = live ? kv_slot(a.pools, pages, kvh, (base + lane) & ((1 << a.pools.page_shift) - 1)) : 0;
-            cp4(st + 2 * kTile * RB + 4 * lane, a.pools.k_scale + slot, live);
-            cp4(st + 2 * kTile * RB + 4 * kTile + 4 * lane, a.pools.v_scale + slot, live);
+            cp4(st + 2 * kTile * RB + 4 * lane, a.pools.k_scale + slot, pages >= 0);
+            cp4(st + 2 * kTile * RB + 4 * kTile + 4 * lane, a.pools.v_scale + slot, pages >= 0);
           }
         }
       }
@@ -368,151 +381,224 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
       pages = page_of(i + 1);
     }
 
+    // ---- this warp's query rows (row r of each n-tile), in fragment order
+    uint32_t qf[NT][KS][2];
+    float row_scale[NT][2];  // of rows 2c and 2c + 1: what their scores are multiplied by
+    int node[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int base = row0 + rg * 8 * NT + nt * 8;
+      const int row = base + r;
+      const bool live = row < row0 + live_rows;
+      const int i = live ? row / a.group : 0;
+      const int head = kvh * a.group + (live ? row - i * a.group : 0);
+      const uint16_t* src = a.q + (s.first + static_cast<long long>(i)) * a.q_stride + head * HD;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = ((ks / WPC) * 4 + c) * DPC + (ks % WPC) * 4;
+        uint2 v = make_uint2(0u, 0u);
+        if (live) v = *reinterpret_cast<const uint2*>(src + d);
+        qf[nt][ks][0] = v.x;
+        qf[nt][ks][1] = v.y;
+      }
+      float up = 1.f;  // (row r's own)
+      if constexpr (CODES) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top = max(top, max(qf[nt][ks][e] & 0x7FFFu, (qf[nt][ks][e] >> 16) & 0x7FFFu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the largest becomes 1 to 2 (2 to 4 at the top of bf16's range)
+        const uint32_t ex = top >> 7, f = min(max(254 - static_cast<int>(ex), 1), 253);
+        const float down = __uint_as_float(f << 23);
+        up = __uint_as_float((254u - f) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[nt][ks][e] = pack_rn_f16x2(bf16lo(qf[nt][ks][e]) * down, bf16hi(qf[nt][ks][e]) * down);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        row_scale[nt][e] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
+        const int mine_row = base + 2 * c + e;
+        node[nt][e] = mine_row < row0 + live_rows ? mine_row / a.group : -1;
+      }
+    }
+
+    float o[DT][NT][4];           // dims r and r + 8 (codes: 2 r and 2 r + 1) of each 16, rows 2c and 2c + 1
+    float m[NT][2], mv[NT][2], l[NT][2];  // maxima of the scores, and with the values' scales; sums
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = mv[nt][e] = kFirstMax;
+        l[nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][nt][e] = 0.f;
+    }
+
     for (int i = 0; i < mine; ++i) {
       cp_wait<NST - 2>();
       group_sync();  // every warp of the group has the tile, and is done with the one before it
       issue(i + NST - 1, pages);
       pages = page_of(i + NST);
-      const uint32_t st = ring + (i % NST) * S::kStageBytes;
+      const uint32_t off = (ring - smem_u32(smem)) + (i % NST) * S::kStageBytes;
+      const uint32_t st = smem_u32(smem) + off;
       const int base = key0 + kTile * (kg + KG * i);
 
-      // ---- S = Q K^T
-      float sc[MT][4][4];
+      // ---- S^T = K Q^T: sc[mt][nt]: keys 16 mt + r (0, 1) and + 8 (2, 3), rows 2c (0, 2) and 2c + 1 (1, 3)
+      float sc[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[mt][n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) sc[mt][nt][e] = 0.f;
 #pragma unroll
-      for (int j = 0; j < CPR / 4; ++j)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint4 w = lds128(st + piece_at<RB>(n * 8 + r, 4 * j + c));
-          const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+        for (int j = 0; j < CPR / 4; ++j) {
+          const uint4 x = lds128(st + piece_at<RB>(mt * 16 + r, 4 * j + c));
+          const uint4 y = lds128(st + piece_at<RB>(mt * 16 + 8 + r, 4 * j + c));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int x = 0; x < WPC; ++x) {
-            uint32_t b0, b1;
-            if constexpr (FMT == NCM_KV_BF16) {
-              b0 = e[2 * x];
-              b1 = e[2 * x + 1];
+          for (int w = 0; w < WPC; ++w) {
+            uint32_t f[4];
+            if constexpr (CODES) {
+              code_pairs<FMT>(xs[w], &f[0], &f[2]);
+              code_pairs<FMT>(ys[w], &f[1], &f[3]);
             } else {
-              b0 = code_pair<FMT, 0, 1>(e[x]);
-              b1 = code_pair<FMT, 2, 3>(e[x]);
+              f[0] = xs[2 * w];
+              f[1] = ys[2 * w];
+              f[2] = xs[2 * w + 1];
+              f[3] = ys[2 * w + 1];
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_bf16(sc[mt][n], qf[mt][j * WPC + x], b0, b1);
+            for (int nt = 0; nt < NT; ++nt) mma16<CODES>(sc[mt][nt], f, qf[nt][j * WPC + w][0], qf[nt][j * WPC + w][1]);
           }
         }
 
       // ---- scores in units of log2, masked where the row does not see the key
-      float2 vs[4];
+      float vlog[2][2];  // log2 of the values' scales of keys 16 mt + 8 h + r
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        float2 f = make_float2(a.scale_log2, a.scale_log2);
-        if constexpr (FMT != NCM_KV_BF16) {
-          const float* scales = reinterpret_cast<const float*>(smem + (st - smem_u32(smem)) + 2 * kTile * RB);
-          const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8 + 2 * c);
-          vs[n] = *reinterpret_cast<const float2*>(scales + kTile + n * 8 + 2 * c);
-          f.x *= ks.x;
-          f.y *= ks.y;
-        }
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          sc[mt][n][0] *= f.x;
-          sc[mt][n][1] *= f.y;
-          sc[mt][n][2] *= f.x;
-          sc[mt][n][3] *= f.y;
+        for (int h = 0; h < 2; ++h) {
+          float ks = 1.f;
+          if constexpr (CODES) {
+            const float* scales = reinterpret_cast<const float*>(smem + off + 2 * kTile * RB) + mt * 16 + h * 8 + r;
+            ks = scales[0];
+            vlog[mt][h] = lg2(scales[kTile]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float t = sc[mt][nt][2 * h + e] * row_scale[nt][e];
+              if constexpr (CODES) t *= ks;
+              sc[mt][nt][2 * h + e] = t;
+            }
         }
-      }
       const bool partly = base + kTile > min(ctx, key1);  // new tokens, or the segment's end, in this tile
-      uint32_t vis[MT][2];
+      uint32_t vis[NT][2];
       if (partly) {
         const uint32_t present = first_bits(key1 - base);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int i2 = node[mt][e];
+            const int i2 = node[nt][e];
             uint32_t w = 0u;
             if (i2 >= 0)
               w = present & (a.mask == nullptr
                                  ? first_bits(ctx + i2 - base + 1)
                                  : mask_window(a.mask + (s.first + static_cast<long long>(i2)) * a.mask_words, a.mask_words, base - ctx));
-            vis[mt][e] = w;
-            w >>= 2 * c;
+            vis[nt][e] = w;
+            w >>= r;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              if (!((w >> (8 * n)) & 1u)) sc[mt][n][2 * e] = -INFINITY;
-              if (!((w >> (8 * n + 1)) & 1u)) sc[mt][n][2 * e + 1] = -INFINITY;
-            }
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (!((w >> (16 * mt + 8 * h)) & 1u)) sc[mt][nt][2 * h + e] = -INFINITY;
           }
       }
 
-      // ---- move the maximum only where a score passes it by more than the slack
+      // ---- move a maximum only where a score passes it by more than the slack
       bool move = false;
-      float top[MT][2];
+      float top[NT][2], topv[NT][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(sc[mt][0][2 * e], sc[mt][0][2 * e + 1]);
-#pragma unroll
-          for (int n = 1; n < 4; ++n) x = fmaxf(x, fmaxf(sc[mt][n][2 * e], sc[mt][n][2 * e + 1]));
-          top[mt][e] = x;
-          move |= x > m[mt][e] + kSlack;
+          top[nt][e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][2 + e]), fmaxf(sc[1][nt][e], sc[1][nt][2 + e]));
+          move |= top[nt][e] > m[nt][e] + kSlack;
+          if constexpr (CODES) {
+            topv[nt][e] = fmaxf(fmaxf(sc[0][nt][e] + vlog[0][0], sc[0][nt][2 + e] + vlog[0][1]),
+                                fmaxf(sc[1][nt][e] + vlog[1][0], sc[1][nt][2 + e] + vlog[1][1]));
+            move |= topv[nt][e] > mv[nt][e] + kSlack;
+          }
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = top[mt][e];
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            x = fmaxf(x, m[mt][e]);
-            const float f = ex2(m[mt][e] - x);
-            m[mt][e] = x;
-            l[mt][e] *= f;
+            float x = top[nt][e];
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) {
-              o[mt][n][2 * e] *= f;
-              o[mt][n][2 * e + 1] *= f;
+            for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
+            x = fmaxf(x, m[nt][e]);
+            float f = ex2(m[nt][e] - x);
+            m[nt][e] = x;
+            l[nt][e] *= f;
+            if constexpr (CODES) {
+              x = topv[nt][e];
+#pragma unroll
+              for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
+              x = fmaxf(x, mv[nt][e]);
+              f = ex2(mv[nt][e] - x);
+              mv[nt][e] = x;
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              o[d][nt][e] *= f;
+              o[d][nt][2 + e] *= f;
             }
           }
       }
 
-      // ---- probabilities: f32 in the sum, bf16 (with the values' scales) in the product
-      uint32_t pf[MT][2][4];
+      // ---- probabilities: f32 in the sum, 16 bits (codes: with the values' scales) in the product
+      uint32_t pf[2][NT][2];  // P^T: keys 16 mt + 2c, + 1 (0) and + 8 (1) of row r
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float p[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2(sc[mt][n][e] - m[mt][e >> 1]);
-          l[mt][0] += p[0] + p[1];
-          l[mt][1] += p[2] + p[3];
-          if constexpr (FMT != NCM_KV_BF16) {
+          for (int h = 0; h < 2; ++h) {
+            float p[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float z = p[e] * (e & 1 ? vs[n].y : vs[n].x);
-              // (a hidden key's scale may be NaN: its row is not to hear of it)
-              p[e] = partly && !((vis[mt][e >> 1] >> (8 * n + 2 * c + (e & 1))) & 1u) ? 0.f : z;
+            for (int e = 0; e < 2; ++e) {
+              const float t = sc[mt][nt][2 * h + e];
+              p[e] = ex2(t - m[nt][e]);
+              l[nt][e] += p[e];
+              if constexpr (CODES) {
+                p[e] = ex2(t + vlog[mt][h] - mv[nt][e]);
+                // (a hidden key's scale may be NaN: its row is not to hear of it)
+                if (partly && !((vis[nt][e] >> (16 * mt + 8 * h + r)) & 1u)) p[e] = 0.f;
+              } else {
+                sc[mt][nt][2 * h + e] = p[e];
+              }
             }
+            pf[mt][nt][h] = transpose8x8(CODES ? pack_rn_f16x2(p[0], p[1]) : pack_rn_bf16x2(p[0], p[1]));
           }
-          pf[mt][n >> 1][(n & 1) * 2] = pack_rn(p[0], p[1]);
-          pf[mt][n >> 1][(n & 1) * 2 + 1] = pack_rn(p[2], p[3]);
-          if constexpr (FMT == NCM_KV_BF16) {
-            sc[mt][n][0] = p[0];
-            sc[mt][n][1] = p[1];
-            sc[mt][n][2] = p[2];
-            sc[mt][n][3] = p[3];
-          }
-        }
 
       const uint32_t vst = st + kTile * RB;
-      if constexpr (FMT == NCM_KV_BF16) {
+      if constexpr (!CODES) {
         // A new token's value row may hold a NaN or an infinity and be hidden from
         // some rows: 0 * NaN would reach them. Such rows are taken out of the tile
         // and added by the rows that see them.
@@ -525,28 +611,30 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
 #pragma unroll
             for (int y = 0; y < 4; ++y) odd |= (e[y] & 0x7F80u) == 0x7F80u || (e[y] & 0x7F800000u) == 0x7F800000u;
           }
-          uint32_t bad = __ballot_sync(0xffffffffu, odd);
+          const uint32_t bad = __ballot_sync(0xffffffffu, odd);
           if (bad != 0u) {
             group_sync();
             for (uint32_t left = bad; left != 0u; left &= left - 1u) {
               const int key = __ffs(left) - 1;
-              const int from = (lane & ~3) | ((key >> 1) & 3);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   float p = 0.f;
 #pragma unroll
-                  for (int n = 0; n < 4; ++n)
-                    if (n == (key >> 3)) p = (key & 1) ? sc[mt][n][2 * e + 1] : sc[mt][n][2 * e];
-                  p = __shfl_sync(0xffffffffu, p, from);
-                  if ((vis[mt][e] >> key) & 1u) {
+                  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int n = 0; n < HD / 8; ++n) {
-                      const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vst - smem_u32(smem)) + piece_at<RB>(key, n) + 4 * c);
-                      o[mt][n][2 * e] = fmaf(p, bf16lo(w), o[mt][n][2 * e]);
-                      o[mt][n][2 * e + 1] = fmaf(p, bf16hi(w), o[mt][n][2 * e + 1]);
-                    }
+                    for (int h = 0; h < 2; ++h)
+                      if (key >> 3 == 2 * mt + h) p = sc[mt][nt][2 * h + e];
+                  p = __shfl_sync(0xffffffffu, p, (key & 7) * 4 + c);
+                  if ((vis[nt][e] >> key) & 1u) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                      for (int h = 0; h < 2; ++h) {
+                        const uint16_t v = *reinterpret_cast<const uint16_t*>(smem + off + kTile * RB + piece_at<RB>(key, 2 * d + h) + 2 * r);
+                        o[d][nt][2 * h + e] = fmaf(p, bf16_to_f32(v), o[d][nt][2 * h + e]);
+                      }
                   }
                 }
             }
@@ -558,81 +646,75 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
         }
       }
 
-      // ---- O += P V
+      // ---- O^T += V^T P^T
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int key = kk * 16 + (lane & 15);
+      for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int x = 0; x < CPR / 2; ++x) {
           uint32_t w[4];
-          ldmatrix_x4_trans(w, vst + piece_at<RB>(key, 2 * x + (lane >> 4)));
-          if constexpr (FMT == NCM_KV_BF16) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma_bf16(o[mt][2 * x], pf[mt][kk], w[0], w[1]);
-              mma_bf16(o[mt][2 * x + 1], pf[mt][kk], w[2], w[3]);
-            }
-          } else {
-            // a 16-bit element is a pair of dims: the even ones, then the odd ones
+          if constexpr (CODES) {  // 16-bit elements are pairs of dims: the even ones become rows r, the odd ones rows r + 8
+            ldmatrix_x4_trans(w, vst + piece_at<RB>(kk * 16 + (lane & 15), 2 * x + (lane >> 4)));
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const uint32_t e0 = code_pair<FMT, 0, 2>(w[2 * y]), e1 = code_pair<FMT, 0, 2>(w[2 * y + 1]);
-              const uint32_t o0 = code_pair<FMT, 1, 3>(w[2 * y]), o1 = code_pair<FMT, 1, 3>(w[2 * y + 1]);
+              uint32_t f[4];
+              code_pairs_strided<FMT>(w[2 * y], &f[0], &f[1]);
+              code_pairs_strided<FMT>(w[2 * y + 1], &f[2], &f[3]);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma_bf16(o[mt][4 * x + 2 * y], pf[mt][kk], e0, e1);
-                mma_bf16(o[mt][4 * x + 2 * y + 1], pf[mt][kk], o0, o1);
-              }
+              for (int nt = 0; nt < NT; ++nt) mma16<true>(o[2 * x + y][nt], f, pf[kk][nt][0], pf[kk][nt][1]);
             }
+          } else {
+            ldmatrix_x4_trans(w, vst + piece_at<RB>(kk * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * x + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16<false>(o[x][nt], w, pf[kk][nt][0], pf[kk][nt][1]);
           }
         }
-      }
     }
     cp_wait<0>();
     __syncthreads();  // the ring's memory now carries the key groups' sums
 
-    // ---- the key groups' sums: [KG][ROWS][m, l, values]
+    // ---- the key groups' sums: [KG][ROWS][m, l, m', -, values]
     constexpr int STR = HD + 4;
     float* mg = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = l[mt][e];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        float* row = mg + (kg * ROWS + rg * 16 * MT + mt * 16 + r + 8 * e) * STR;
-        if (c == 0) {
-          row[0] = m[mt][e];
-          row[1] = x;
-        }
+        float x = l[nt][e];
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {
-          if constexpr (FMT == NCM_KV_BF16) {
-            *reinterpret_cast<float2*>(row + 4 + n * 8 + 2 * c) = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
-          } else if (n % 2 == 0) {
-            *reinterpret_cast<float4*>(row + 4 + (n / 2) * 16 + 4 * c) =
-                make_float4(o[mt][n][2 * e], o[mt][n + 1][2 * e], o[mt][n][2 * e + 1], o[mt][n + 1][2 * e + 1]);
+        for (int z = 4; z < 32; z <<= 1) x += __shfl_xor_sync(0xffffffffu, x, z);
+        float* row = mg + (kg * ROWS + rg * 8 * NT + nt * 8 + 2 * c + e) * STR;
+        if (r == 0) *reinterpret_cast<float4*>(row) = make_float4(m[nt][e], x, CODES ? mv[nt][e] : m[nt][e], 0.f);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if constexpr (CODES) {
+            *reinterpret_cast<float2*>(row + 4 + 16 * d + 2 * r) = make_float2(o[d][nt][e], o[d][nt][2 + e]);
+          } else {
+            row[4 + 16 * d + r] = o[d][nt][e];
+            row[4 + 16 * d + 8 + r] = o[d][nt][2 + e];
           }
         }
       }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == units;
-    float* part = a.part + (2ll * blockIdx.x + (u0 == 0 ? 1 : 0)) * ROWS * (HD + 2);
+    float* part = a.part + (2ll * blockIdx.x + (u0 == 0 ? 1 : 0)) * ROWS * STR;
     const int rows = min(ROWS, live_rows);
     for (int x = threadIdx.x; x < rows * (HD / 4); x += S::kThreads) {
       const int row = x / (HD / 4), d = (x % (HD / 4)) * 4;
-      float mm = kFirstMax;
+      float4 top = *reinterpret_cast<const float4*>(mg + row * STR);
 #pragma unroll
-      for (int k = 0; k < KG; ++k) mm = fmaxf(mm, mg[(k * ROWS + row) * STR]);
+      for (int k = 1; k < KG; ++k) {
+        const float* src = mg + (k * ROWS + row) * STR;
+        top.x = fmaxf(top.x, src[0]);
+        top.z = fmaxf(top.z, src[2]);
+      }
       float sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < KG; ++k) {
         const float* src = mg + (k * ROWS + row) * STR;
-        const float f = ex2(src[0] - mm);
+        const float f = ex2(src[2] - top.z);
         const float4 y = *reinterpret_cast<const float4*>(src + 4 + d);
-        sum = fmaf(src[1], f, sum);
+        sum = fmaf(src[1], ex2(src[0] - top.x), sum);
         v.x = fmaf(y.x, f, v.x);
         v.y = fmaf(y.y, f, v.y);
         v.z = fmaf(y.z, f, v.z);
@@ -641,16 +723,15 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
       if (whole) {
         const int i = (row0 + row) / a.group, head = kvh * a.group + (row0 + row) - i * a.group;
         const long long t = s.first + static_cast<long long>(i);
-        const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
+        const float f = out_factor(sum, top.z - top.x);
+        const float g = half_power(top.z - top.x);
         *reinterpret_cast<uint2*>(a.out + t * a.out_stride + head * HD + d) =
-            sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
-        if (d == 0 && a.lse != nullptr)
-          a.lse[t * a.heads + head] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * 0.69314718055994531f;
+            make_uint2(pack_rn_bf16x2(v.x * f * g, v.y * f * g), pack_rn_bf16x2(v.z * f * g, v.w * f * g));
+        if (d == 0 && a.lse != nullptr) a.lse[t * a.heads + head] = lse_of(top.x, sum);
       } else {
-        float* dst = part + row * (HD + 2);
-        if (d == 0) *reinterpret_cast<float2*>(dst) = make_float2(mm, sum);
-        *reinterpret_cast<float2*>(dst + 2 + d) = make_float2(v.x, v.y);
-        *reinterpret_cast<float2*>(dst + 4 + d) = make_float2(v.z, v.w);
+        float* dst = part + row * STR;
+        if (d == 0) *reinterpret_cast<float4*>(dst) = make_float4(top.x, sum, top.z, 0.f);
+        *reinterpret_cast<float4*>(dst + 4 + d) = v;
       }
     }
     __syncthreads();
@@ -667,7 +748,8 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int R
   pdl_wait();
   pdl_launch_dependents();
   constexpr int DPL = HD / 32;
-  __shared__ float sh[4][HD + 2];
+  constexpr int STR = HD + 4;
+  __shared__ float sh[4][STR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / a.pools.kv_heads, kvh = blockIdx.x - b * a.pools.kv_heads;
   const Seq s = load_seq(a, b, false);
@@ -691,48 +773,40 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int R
   const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units, x1 = x0 + units - 1;
   const int c0 = static_cast<int>(((x0 + 1) * a.grid - 1) / all), c1 = static_cast<int>(((x1 + 1) * a.grid - 1) / all);
   if (c0 == c1) return;
-  float mm = kFirstMax, sum = 0.f, v[DPL];
+  float mm = kFirstMax, mv = kFirstMax, sum = 0.f, v[DPL];
 #pragma unroll
   for (int d = 0; d < DPL; ++d) v[d] = 0.f;
-  auto add = [&](float m2, float l2, const float* y) {
-    const float top = fmaxf(mm, m2);
-    const float f = ex2(mm - top), g = ex2(m2 - top);
-    sum = sum * f + l2 * g;
+  auto add = [&](const float* src) {
+    const float top = fmaxf(mm, src[0]), topv = fmaxf(mv, src[2]);
+    sum = sum * ex2(mm - top) + src[1] * ex2(src[0] - top);
+    const float f = ex2(mv - topv), g = ex2(src[2] - topv);
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) v[d] = v[d] * f + y[d] * g;
+    for (int d = 0; d < DPL; ++d) v[d] = v[d] * f + src[4 + lane + 32 * d] * g;
     mm = top;
+    mv = topv;
   };
   for (int c = c0 + warp; c <= c1; c += 4) {
-    const float* src = a.part + ((2ll * c + (c == c0 ? 1 : 0)) * ROWS + row) * (HD + 2);
-    // (CTAs of a grid larger than the number of units have none between c0 and c1)
+    // (a grid larger than the number of units has CTAs without any between c0 and c1)
     if (all * c / a.grid == all * (c + 1) / a.grid) continue;
-    float y[DPL];
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) y[d] = src[2 + lane + 32 * d];
-    add(src[0], src[1], y);
+    add(a.part + ((2ll * c + (c == c0 ? 1 : 0)) * ROWS + row) * STR);
   }
   if (lane == 0) {
     sh[warp][0] = mm;
     sh[warp][1] = sum;
+    sh[warp][2] = mv;
   }
 #pragma unroll
-  for (int d = 0; d < DPL; ++d) sh[warp][2 + lane + 32 * d] = v[d];
+  for (int d = 0; d < DPL; ++d) sh[warp][4 + lane + 32 * d] = v[d];
   __syncthreads();
   if (warp != 0) return;
-  for (int w = 1; w < 4; ++w) {
-    float y[DPL];
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) y[d] = sh[w][2 + lane + 32 * d];
-    add(sh[w][0], sh[w][1], y);
-  }
+  for (int w = 1; w < 4; ++w) add(sh[w]);
   const int i = row_all / a.group, head = kvh * a.group + row_all - i * a.group;
   const long long t = s.first + static_cast<long long>(i);
-  const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
+  const float f = out_factor(sum, mv - mm), g = half_power(mv - mm);
 #pragma unroll
   for (int d = 0; d < DPL; ++d)
-    a.out[t * a.out_stride + head * HD + lane + 32 * d] = sum == 0.f ? 0 : f32_to_bf16(v[d] * inv);
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[t * a.heads + head] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * 0.69314718055994531f;
+    a.out[t * a.out_stride + head * HD + lane + 32 * d] = static_cast<uint16_t>(pack_rn_bf16x2(v[d] * f * g, 0.f));
+  if (lane == 0 && a.lse != nullptr) a.lse[t * a.heads + head] = lse_of(mm, sum);
 }
 
 using TreeKernel = void (*)(const TreeArgs);
@@ -740,21 +814,21 @@ struct Variant {
   TreeKernel kernel;
   int rows, threads, smem;
 };
-template <int HD, int FMT, int MT, int RG, int KG>
+template <int HD, int FMT, int NT, int RG, int KG>
 constexpr Variant variant() {
-  using S = TreeShape<HD, FMT, MT, RG, KG>;
-  return Variant{tree_attention_kernel<HD, FMT, MT, RG, KG>, S::kRows, S::kThreads, S::kSmem};
+  using S = TreeShape<HD, FMT, NT, RG, KG>;
+  return Variant{tree_attention_kernel<HD, FMT, NT, RG, KG>, S::kRows, S::kThreads, S::kSmem};
 }
 
-// By the rows of one kv head: few rows take the keys four groups at a time, many
-// share each tile among four row groups.
-constexpr int kSizes = 4;
+// By the rows of one kv head: 8, 16, 32, 64 or 128 rows a tile. Few rows take
+// the keys four groups at a time, many share each tile among four row groups.
+constexpr int kSizes = 5;
 template <int FMT>
 struct Variants {
-  static constexpr Variant hd64[kSizes] = {variant<64, FMT, 1, 1, 4>(), variant<64, FMT, 2, 1, 4>(), variant<64, FMT, 2, 2, 2>(),
-                                           variant<64, FMT, 2, 4, 1>()};
-  static constexpr Variant hd128[kSizes] = {variant<128, FMT, 1, 1, 4>(), variant<128, FMT, 1, 2, 2>(), variant<128, FMT, 1, 4, 1>(),
-                                            variant<128, FMT, 1, 4, 1>()};
+  static constexpr Variant hd64[kSizes] = {variant<64, FMT, 1, 1, 4>(), variant<64, FMT, 2, 1, 4>(), variant<64, FMT, 4, 1, 4>(),
+                                           variant<64, FMT, 4, 2, 2>(), variant<64, FMT, 4, 4, 1>()};
+  static constexpr Variant hd128[kSizes] = {variant<128, FMT, 1, 1, 4>(), variant<128, FMT, 2, 1, 4>(), variant<128, FMT, 2, 2, 2>(),
+                                            variant<128, FMT, 2, 4, 1>(), variant<128, FMT, 2, 4, 1>()};
 };
 
 const Variant& pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
@@ -762,7 +836,7 @@ const Variant& pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
   const Variant* v = c->format == NCM_KV_BF16   ? (wide ? Variants<NCM_KV_BF16>::hd128 : Variants<NCM_KV_BF16>::hd64)
                      : c->format == NCM_KV_INT8 ? (wide ? Variants<NCM_KV_INT8>::hd128 : Variants<NCM_KV_INT8>::hd64)
                                                 : (wide ? Variants<NCM_KV_E4M3>::hd128 : Variants<NCM_KV_E4M3>::hd64);
-  const int i = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+  const int i = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 3 : 4;
   *index = (c->format * 2 + wide) * kSizes + i;
   return v[i];
 }
@@ -804,7 +878,7 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
   p->merge = cap > kWholeKeys;
   p->unit_keys = p->merge ? kUnitKeys : static_cast<int>(kWholeKeys);
   p->grid = ctx->num_sms * resident[index].load();
-  p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 2) * sizeof(float);
+  p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
   return NCM_OK;
 }
 

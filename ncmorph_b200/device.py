@@ -43,6 +43,13 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(device: torch.device) -> int:
+    """Handle of torch's current stream on a device (the C ABI's stream argument),
+    without the stream object that stream_of makes: 0.1 instead of 2.7 us, which
+    counts where a call's kernel takes a few microseconds."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p | None:
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
@@ -62,35 +69,38 @@ def need(t: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple | None = N
     return t
 
 
-def need_rows(t: torch.Tensor, dtype: torch.dtype, name: str, device: torch.device, width: int) -> int:
-    """Validates a [rows, >= width] matrix whose rows may be strided (a column
-    slice of a wider matrix, say) and returns its row stride in elements."""
+def _need_tensor(t: torch.Tensor, dtype: torch.dtype, name: str, device: torch.device) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dim() != 2 or t.shape[1] < width:
-        raise ValueError(f"{name} must be a matrix of at least {width} columns, got {tuple(t.shape)}")
-    rows, stride = t.shape[0], t.stride(0)
-    if t.stride(1) != 1 or (rows > 1 and stride < t.shape[1]):
+
+
+def need_rows(t: torch.Tensor, dtype: torch.dtype, name: str, device: torch.device, width: int) -> int:
+    """Validates a [rows, >= width] matrix whose rows may be strided (a column
+    slice of a wider matrix, say) and returns its row stride in elements."""
+    _need_tensor(t, dtype, name, device)
+    shape = t.shape
+    if len(shape) != 2 or shape[1] < width:
+        raise ValueError(f"{name} must be a matrix of at least {width} columns, got {tuple(shape)}")
+    stride, inner = t.stride()
+    rows, cols = shape
+    if rows <= 1:  # a single row's stride says nothing: the row itself covers what is read
+        stride = max(stride, cols + 7 & ~7)
+    if (inner != 1 and cols > 1) or stride < cols:
         raise ValueError(f"{name} must have contiguous, separate rows")
-    # (a single row's stride says nothing: the row itself covers what is read)
-    return stride if rows > 1 else max(stride, t.shape[1] + 7 & ~7)
+    return stride
 
 
 def need_vec(t: torch.Tensor | None, dtype: torch.dtype, name: str, device: torch.device, n: int | None = None):
     """Address of a contiguous vector argument (0 for None), validated."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+    _need_tensor(t, dtype, name, device)
+    shape = t.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n) or (shape[0] > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous vector{'' if n is None else f' of {n}'}, got {tuple(t.shape)}")
     return t.data_ptr()
 

@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import context, need_rows, need_vec, stream_of
+from .device import context, need_rows, need_vec, raw_stream
 
 bf16, i32 = torch.bfloat16, torch.int32
 FORMATS = {bf16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
@@ -99,7 +99,7 @@ def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, token_start: torch.
         raise ValueError(f"k and v must have the same rows, got {k.shape[0]} and {v.shape[0]}")
     b = _batch(cache, token_start, kv_lens, page_table, k.shape[0])
     _lib.call("ncm_kv_cache_append", context(dev), cache._ref, ctypes.byref(b), k.data_ptr(), ks, v.data_ptr(), vs,
-              stream_of(k))
+              raw_stream(dev))
 
 
 def gather(cache: KVCache, row_start: torch.Tensor, page_table: torch.Tensor, rows: int | None = None,
@@ -120,7 +120,7 @@ def gather(cache: KVCache, row_start: torch.Tensor, page_table: torch.Tensor, ro
         raise ValueError("out_k and out_v must have the same rows")
     b = _batch(cache, row_start, None, page_table, out_k.shape[0])
     _lib.call("ncm_kv_cache_gather", context(dev), cache._ref, ctypes.byref(b),
-              need_vec(begin, i32, "begin", dev, b.batch), out_k.data_ptr(), ks, out_v.data_ptr(), vs, stream_of(out_k))
+              need_vec(begin, i32, "begin", dev, b.batch), out_k.data_ptr(), ks, out_v.data_ptr(), vs, raw_stream(dev))
     return out_k, out_v
 
 
@@ -162,5 +162,5 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     _lib.call("ncm_tree_attention", ctx, cache._ref, bref, q.data_ptr(), qs,
               None if tree_mask is None else tree_mask.data_ptr(), words, heads, max_nodes,
               hd ** -0.5 if scale is None else scale, out.data_ptr(), os_, None if lse is None else lse.data_ptr(),
-              None if ws is None else ws.data_ptr(), size.value, stream_of(q))
+              None if ws is None else ws.data_ptr(), size.value, raw_stream(dev))
     return (out, lse) if return_lse else out

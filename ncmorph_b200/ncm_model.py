@@ -15,10 +15,11 @@ import numpy as np
 import torch
 
 from . import _lib
-from .device import context, need, need_rows, need_vec, ptr, stream_of
+from .device import context, need, need_rows, need_vec, ptr, raw_stream, stream_of
 
 MASK_MODES = {"causal": 0, "block_diagonal": 1, "block_causal": 2}
 bf16 = torch.bfloat16
+LOGIT_TYPES = {torch.float32: 2, bf16: 0}  # NCM_DTYPE_F32, NCM_DTYPE_BF16
 
 
 def make_mask(mode: str, prefix_length: int = 0, level_lengths=(), prefix_pad=(),
@@ -83,10 +84,9 @@ def rope_bf16(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: 
     stride = need_rows(x, bf16, "x", dev, width)
     T = x.shape[0]
     P, rotary = cos.shape
-    need(cos, torch.float32, "cos")
-    need(sin, torch.float32, "sin", (P, rotary))
-    if cos.device != dev or sin.device != dev:
-        raise ValueError(f"cos and sin must be on {dev}")
+    if need_rows(cos, torch.float32, "cos", dev, rotary) != rotary and P > 1 or sin.shape != cos.shape or \
+            need_rows(sin, torch.float32, "sin", dev, rotary) != rotary and P > 1:
+        raise ValueError(f"cos and sin must be contiguous and of one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
     pos = need_vec(positions, torch.int32, "positions", dev, T)
     if out is None:
         out = torch.empty((T, width), dtype=bf16, device=dev)
@@ -94,7 +94,7 @@ def rope_bf16(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: 
     if out.shape[0] != T:
         raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
     _lib.call("ncm_rope_bf16", context(dev), x.data_ptr(), stride, out.data_ptr(), out_stride, pos, cos.data_ptr(),
-              sin.data_ptr(), P, T, heads, head_dim, rotary, int(interleaved), int(inverse), stream_of(x))
+              sin.data_ptr(), P, T, heads, head_dim, rotary, interleaved, inverse, raw_stream(dev))
     return out
 
 
@@ -342,7 +342,6 @@ def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, tok
         r.allowed_rows = need_vec(allowed_rows, i32, "allowed_rows", dev, R)
     elif allowed_rows is not None:
         raise ValueError("allowed_rows needs allowed")
-    types = {f32: 2, bf16: 0}
-    _lib.call("ncm_logits_process", context(dev), logits.data_ptr(), types[logits.dtype], stride, out.data_ptr(),
-              types[out.dtype], out_stride, R, V, ctypes.byref(r), stream_of(logits))
+    _lib.call("ncm_logits_process", context(dev), logits.data_ptr(), LOGIT_TYPES[logits.dtype], stride, out.data_ptr(),
+              LOGIT_TYPES[out.dtype], out_stride, R, V, ctypes.byref(r), raw_stream(dev))
     return out
