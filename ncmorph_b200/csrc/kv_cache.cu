@@ -8,7 +8,7 @@
 // by 2^-16 or more, relative to itself: M x and A have at most 15 and 8
 // significant bits, so their nonzero differences from a halfway point are
 // whole units of at most 16 bits (13 for e4m3, whose halfway points have 5 bits).
-// x * fl(M / A) is off by 2^-23 at most. Rounded to 18 bits (Veltkamp's splitting) it is
+// x * (M * rcp(A)) is off by 2^-21 at most. Rounded to 18 bits (Veltkamp's splitting) it is
 // halfway exactly where the quotient is, so the codes are those of exact
 // arithmetic, ties included, without a division per value.
 //
@@ -45,42 +45,42 @@ __device__ __forceinline__ float2 f16x2_to_f32(uint32_t v) {
 
 // The largest magnitude of a row held by LPR lanes, as bf16 bits (they order as integers).
 template <int LPR>
-__device__ __forceinline__ uint32_t row_top(uint32_t top) {
+__device__ __forceinline__ uint32_t row_top(const uint4& v) {
+  uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  return top;
-}
-__device__ __forceinline__ uint32_t top_of(const uint4& v) {
-  const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(e[i] & 0x7FFFu, (e[i] >> 16) & 0x7FFFu));
-  return top;
+  for (int o = LPR / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return max(top >> 16, top & 0xFFFFu);
 }
 
-// M / A for a row whose largest magnitude is `top`, and the power of two that
-// its values are multiplied by first (so that neither over- nor underflows).
+// Eight values of a row whose largest magnitude is `top` -> their codes and the row's scale.
 template <int FMT>
-__device__ __forceinline__ float code_factor(uint32_t top, float* pre) {
+__device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top, float* scale) {
   constexpr float M = FMT == NCM_KV_INT8 ? 127.f : 448.f;
-  *pre = top < 0x1000u ? 0x1p64f : 1.f;
-  if (top >= 0x7F80u || top == 0u) return 0.f;
-  return __fdiv_rn(M, __uint_as_float(top << 16) * *pre);
-}
-
-// Eight values of a row -> their codes. zero: a row without finite largest magnitude.
-template <int FMT>
-__device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top) {
-  float pre;
-  const float factor = code_factor<FMT>(top, &pre);
-  if (factor == 0.f) return make_uint2(0u, 0u);
   const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-  float y[8];
+  const float big = __uint_as_float(top << 16);
+  float y[8], factor;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (i & 1) ? bf16hi(e[i >> 1]) : bf16lo(e[i >> 1]);
+  if (top - 0x1000u < 0x6E80u) {  // 2^-95 <= A < 2^126: 1 / A and M / A are normal numbers
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(big));
+    factor = M * inv;
+    // A / M: one correction by the exact remainder rounds it correctly (A has 128 mantissas)
+    const float q = big * (1.f / M);
+    *scale = fmaf(fmaf(-q, M, big), 1.f / M, q);
+  } else if (top == 0u || top >= 0x7F80u) {  // zeros; a NaN or an infinity
+    *scale = top == 0u ? 1.f : __uint_as_float(0x7FC00000u);
+    return make_uint2(0u, 0u);
+  } else {
+    const float pre = top < 0x1000u ? 0x1p64f : 0x1p-32f;
+    *scale = __fdiv_rn(big, M);
+    factor = __fdiv_rn(M, big * pre);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= pre;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = (i & 1) ? bf16hi(e[i >> 1]) : bf16lo(e[i >> 1]);
-    const float q = __fmul_rn(__fmul_rn(x, pre), factor);
-    const float c = __fmul_rn(q, 65.f);
+    const float q = __fmul_rn(y[i], factor), c = __fmul_rn(q, 65.f);
     y[i] = __fsub_rn(c, __fsub_rn(c, q));  // q rounded to 18 bits
   }
   uint32_t out[2];
@@ -96,12 +96,6 @@ __device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top) {
     }
   }
   return make_uint2(out[0], out[1]);
-}
-
-template <int FMT>
-__device__ __forceinline__ float scale_of(uint32_t top) {
-  if (top >= 0x7F80u) return __uint_as_float(0x7FC00000u);
-  return top == 0u ? 1.f : __fdiv_rn(__uint_as_float(top << 16), FMT == NCM_KV_INT8 ? 127.f : 448.f);
 }
 
 template <int FMT>
@@ -180,7 +174,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
   pdl_wait();
   pdl_launch_dependents();
   constexpr bool CODES = FMT != NCM_KV_BF16;
-  constexpr int LPR = HD / 8, EB = CODES ? 1 : 2, BATCH = 4;
+  constexpr int LPR = HD / 8, EB = CODES ? 1 : 2, BATCH = APPEND ? 4 : 8;
   const long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
   for (int i = threadIdx.x; i < a.tokens; i += kRowThreads) slots[i] = slot_of_row<APPEND>(a, t0 + i);
   __syncthreads();
@@ -220,10 +214,11 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
     for (int k = 0; k < BATCH; ++k) {
       uint16_t* row = rows + (i0 + k * step + first) * stride;
       if constexpr (APPEND && CODES) {
-        const uint32_t top = row_top<LPR>(top_of(x[k]));
+        const uint32_t top = row_top<LPR>(x[k]);
         if (at[k] >= 0) {
-          *reinterpret_cast<uint2*>(codes + at[k] * HD) = quantise8<FMT>(x[k], top);
-          if (piece == 0) scales[at[k]] = scale_of<FMT>(top);
+          float sc;
+          *reinterpret_cast<uint2*>(codes + at[k] * HD) = quantise8<FMT>(x[k], top, &sc);
+          if (piece == 0) scales[at[k]] = sc;
         }
       } else if (at[k] >= 0) {
         if constexpr (APPEND)

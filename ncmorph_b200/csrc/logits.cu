@@ -20,8 +20,10 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 constexpr uint32_t kInPrompt = 0x80000000u;
-constexpr uint32_t kNoEntry = 0xFFFFFFFFu;
-constexpr uint32_t kRepeated = 0x80000000u;  // more than one bias entry of this token
+// A token's bias entries: 0 none; otherwise 2^31 - 1 minus the first one's place
+// (larger is earlier), and this bit where there are more.
+constexpr uint32_t kRepeated = 0x80000000u;
+constexpr uint32_t kFirstEntry = 0x7FFFFFFFu;
 
 struct LogitArgs {
   const void* in;
@@ -92,7 +94,7 @@ __device__ __forceinline__ void store8(uint16_t* p, int left, const float (&x)[8
 
 // GROUPS of eight neighbouring tokens a thread.
 template <typename TI, typename TO, bool VEC, int GROUPS>
-__global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs a) {
   extern __shared__ __align__(16) uint32_t sh[];
   pdl_wait();
   pdl_launch_dependents();
@@ -118,9 +120,7 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) 
   }
   if (biased) {
     row_range(R.bias_start, R.num_bias, r, &b_lo, &b_hi, a.err);
-    if (b_hi > b_lo)
-      for (int i = threadIdx.x; i < slice / 4; i += threads)
-        reinterpret_cast<uint4*>(entry)[i] = make_uint4(kNoEntry, kNoEntry, kNoEntry, kNoEntry);
+    for (int i = threadIdx.x; i < slice / 4; i += threads) reinterpret_cast<uint4*>(entry)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   // (everything that is one load away is asked for before the first wait)
   const int prompt = history && R.prompt_lens != nullptr ? __ldg(R.prompt_lens + r) : 0;
@@ -145,34 +145,32 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) 
     }
   }
   __syncthreads();
+  const unsigned first = static_cast<unsigned>(v0), un = static_cast<unsigned>(n);
+  const int t_mid = t_lo + min(max(prompt, 0), t_hi - t_lo);
+  bool bad = false;
 #pragma unroll 4
   for (int i = t_lo + threadIdx.x; i < t_hi; i += threads) {
-    const int id = __ldg(R.tokens + i);
-    const long long j = id - v0;
-    if (id < 0 || id >= a.vocab) {
-      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
-    } else if (j >= 0 && j < n) {
-      if (i - t_lo < prompt)
+    const unsigned id = static_cast<unsigned>(__ldg(R.tokens + i)), j = id - first;
+    if (j < un) {
+      if (i < t_mid)
         atomicOr(count + j, kInPrompt);
       else
         atomicAdd(count + j, 1u);
     }
+    bad |= id >= static_cast<unsigned>(a.vocab);
   }
-  // the first entry of each token, and whether there are more
+  // the first entry of each token, then whether there are more
   for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
-    const int id = __ldg(R.bias_ids + i);
-    const long long j = id - v0;
-    if (id < 0 || id >= a.vocab) {
-      if (blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
-    } else if (j >= 0 && j < n) {
-      atomicMin(entry + j, static_cast<uint32_t>(i - b_lo));
-    }
+    const unsigned id = static_cast<unsigned>(__ldg(R.bias_ids + i)), j = id - first;
+    if (j < un) atomicMax(entry + j, kFirstEntry - static_cast<unsigned>(i - b_lo));
+    bad |= id >= static_cast<unsigned>(a.vocab);
   }
+  if (bad && blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
   __syncthreads();
   if (b_hi > b_lo) {
     for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
-      const long long j = __ldg(R.bias_ids + i) - v0;
-      if (j >= 0 && j < n && (entry[j] & ~kRepeated) != static_cast<uint32_t>(i - b_lo)) atomicOr(entry + j, kRepeated);
+      const unsigned j = static_cast<unsigned>(__ldg(R.bias_ids + i)) - first;
+      if (j < un && (entry[j] & ~kRepeated) != kFirstEntry - static_cast<unsigned>(i - b_lo)) atomicOr(entry + j, kRepeated);
     }
     __syncthreads();
   }
@@ -189,10 +187,10 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           // l / rep as l * (1 / rep): within an f32 rounding, a third of the instructions
-          float y = __fmul_rn(x[g][e], x[g][e] > 0.f ? inv : rep);
-          const uint32_t made = c[e] & ~kInPrompt;
-          if (made != 0u) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(made))), pres);
-          if (c[e] != 0u) x[g][e] = y;
+          const float y = __fmul_rn(x[g][e], x[g][e] > 0.f ? inv : rep);
+          const float made = static_cast<float>(c[e] & ~kInPrompt);
+          const float z = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, made)), pres);
+          x[g][e] = c[e] == 0u ? x[g][e] : c[e] == kInPrompt ? y : z;
         }
       }
     }
@@ -200,14 +198,16 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const LogitArgs a) 
       uint32_t c[8];
       *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(entry + i);
       *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(entry + i + 4);
+      if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0u) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (c[e] == kNoEntry) continue;
-        const int at = b_lo + static_cast<int>(c[e] & ~kRepeated);
-        x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + at));
-        if (c[e] & kRepeated)
-          for (int k = at + 1; k < b_hi; ++k)
-            if (__ldg(R.bias_ids + k) == v0 + i + e) x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + k));
+        for (int e = 0; e < 8; ++e) {
+          if (c[e] == 0u) continue;
+          const int at = b_lo + static_cast<int>(kFirstEntry - (c[e] & ~kRepeated));
+          x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + at));
+          if (c[e] & kRepeated)
+            for (int k = at + 1; k < b_hi; ++k)
+              if (__ldg(R.bias_ids + k) == v0 + i + e) x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + k));
+        }
       }
     }
 #pragma unroll

@@ -36,38 +36,13 @@
 // slots of such items up, in order.
 #include <algorithm>
 
-#include "kv_cache.cuh"
+#include "tree_attention.cuh"
 
 namespace ncm {
 namespace {
 
-constexpr int kTile = 32;        // keys of one ring stage
-constexpr float kFirstMax = -1e30f;
-constexpr float kSlack = 8.f;    // scores may pass the running maximum by 2^8
+constexpr int kTile = 32;  // keys of one ring stage
 
-struct TreeArgs {
-  KvPools pools;
-  KvBatch batch;
-  const uint16_t* q;
-  long long q_stride;
-  const uint32_t* mask;
-  int mask_words;
-  int heads, group, max_nodes;
-  float scale_log2;
-  uint16_t* out;
-  long long out_stride;
-  float* lse;
-  float* part;  // [2 * grid][ROWS][4 + HD]: m, sum of p, m', -, values
-  int unit_keys;
-  int grid;  // CTAs of the attention kernel
-  int* err;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // c += A B, m16n8k16; HALF: f16 operands, otherwise bf16.
 template <bool HALF>
@@ -95,154 +70,16 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// 16 (4) bytes from global to shared memory, zeros where !live.
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint32_t pack_rn_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Four codes as two pairs of f16, exactly: bytes (0, 1) and (2, 3).
-template <int FMT>
-__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t* lo, uint32_t* hi) {
-  if constexpr (FMT == NCM_KV_INT8) {
-    w ^= 0x80808080u;  // 128 + code; 0x6400 | b is 1024 + b
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*lo) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*hi) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
-  } else {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(*lo), "=r"(*hi)
-        : "r"(w));
-  }
-}
-// The same of bytes (0, 2) and (1, 3).
-template <int FMT>
-__device__ __forceinline__ void code_pairs_strided(uint32_t w, uint32_t* even, uint32_t* odd) {
-  if constexpr (FMT == NCM_KV_INT8) {
-    w ^= 0x80808080u;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*even) : "r"(__byte_perm(w, 0x64646464u, 0x4240)), "r"(0x64806480u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*odd) : "r"(__byte_perm(w, 0x64646464u, 0x4341)), "r"(0x64806480u));
-  } else {
-    code_pairs<FMT>(__byte_perm(w, 0u, 0x3120), even, odd);
-  }
-}
-
-// What one sequence contributes: its nodes (0 where its numbers do not fit), keys and units.
-struct Seq {
-  int first, n, len;
-};
-__device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, bool report) {
-  Seq s;
-  s.first = __ldg(a.batch.token_start + b);
-  s.n = __ldg(a.batch.token_start + b + 1) - s.first;
-  s.len = __ldg(a.batch.kv_lens + b);
-  const bool bad = s.first < 0 || s.n < 0 || s.n > a.max_nodes || s.len < s.n ||
-                   static_cast<long long>(s.first) + s.n > a.batch.rows ||
-                   s.len > (static_cast<long long>(a.batch.table_width) << a.pools.page_shift);
-  if (bad) {
-    if (report) atomicOr(a.err, kErrBadIndex);
-    s.n = s.len = 0;
-  }
-  return s;
-}
-
-template <int ROWS>
-__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) {
-  return (s.n * a.group + ROWS - 1) / ROWS;
-}
-__device__ __forceinline__ int units_of(const TreeArgs& a, const Seq& s) { return (s.len + a.unit_keys - 1) / a.unit_keys; }
-
-// Units in front of sequence `upto` (whole warps; every lane gets the sum).
-template <int ROWS>
-__device__ __forceinline__ long long units_before(const TreeArgs& a, int upto) {
-  long long sum = 0;
-  for (int b = threadIdx.x & 31; b < upto; b += 32) {
-    const Seq s = load_seq(a, b, false);
-    sum += static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
-}
-
-// The sequence that holds unit x < total, and the unit's place in it.
-template <int ROWS>
-__device__ __forceinline__ int find_unit(const TreeArgs& a, long long x, long long* inside) {
-  const int lane = threadIdx.x & 31;
-  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
-    long long u = 0;
-    if (b0 + lane < a.batch.batch) {
-      const Seq s = load_seq(a, b0 + lane, false);
-      u = static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
-    }
-    long long before = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += y;
-    }
-    const long long all = __shfl_sync(0xffffffffu, before, 31);
-    before -= u;
-    if (x < all) {
-      const unsigned hit = __ballot_sync(0xffffffffu, x >= before && x < before + u);
-      const int who = __ffs(hit) - 1;
-      *inside = x - __shfl_sync(0xffffffffu, before, who);
-      return b0 + who;
-    }
-    x -= all;
-  }
-  *inside = 0;
-  return a.batch.batch;
-}
-
-// Bits [j0, j0 + 32) of a node's mask row (bits in front of 0 are ones, behind the row zeros).
-__device__ __forceinline__ uint32_t mask_window(const uint32_t* row, int words, int j0) {
-  if (j0 <= -32) return 0xFFFFFFFFu;
-  if (j0 < 0) {
-    const uint32_t w = words > 0 ? __ldg(row) : 0u;
-    return (w << -j0) | ((1u << -j0) - 1u);
-  }
-  const int i = j0 >> 5;
-  const uint32_t lo = i < words ? __ldg(row + i) : 0u, hi = i + 1 < words ? __ldg(row + i + 1) : 0u;
-  return __funnelshift_r(lo, hi, j0 & 31);
-}
-__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
-
 template <int HD, int FMT, int NT, int RG, int KG>
 struct TreeShape {
   static constexpr int kThreads = 32 * RG * KG;
   static constexpr int kRows = 8 * NT * RG;
   static constexpr int kRowBytes = HD * (FMT == NCM_KV_BF16 ? 2 : 1);
   static constexpr int kStageBytes = 2 * kTile * kRowBytes + (FMT == NCM_KV_BF16 ? 0 : 2 * kTile * 4);
-  // two tiles in flight beside the one in use
+  // three stages: two tiles in flight beside the one in use
   static constexpr int kStages = 3;
+  // Eight rows of 64: held to 128 registers, so that four CTAs fit an SM.
+  static constexpr int kMinBlocks = NT == 1 && HD == 64 ? 4 : 1;
   static constexpr int kRingBytes = KG * kStages * kStageBytes;
   static constexpr int kMergeBytes = KG * kRows * (HD + 4) * 4;
   static constexpr int kSmem = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
@@ -259,17 +96,8 @@ __device__ __forceinline__ uint32_t piece_at(int key, int chunk) {
     return key * RB + ((chunk ^ (((key & 1) << 2) | ((key >> 1) & 3))) << 4);
 }
 
-// 2^(d / 2), twice: the values' sums are brought from their maximum to the
-// scores' by 2^d, which alone may pass f32's range.
-__device__ __forceinline__ float half_power(float d) { return ex2(0.5f * d); }
-// half_power(d) / sum; 0 for a row that saw nothing.
-__device__ __forceinline__ float out_factor(float sum, float d) { return sum == 0.f ? 0.f : __fdiv_rn(half_power(d), sum); }
-__device__ __forceinline__ float lse_of(float m, float sum) {
-  return sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
-}
-
 template <int HD, int FMT, int NT, int RG, int KG>
-__global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::kMinBlocks) tree_attention_kernel(const TreeArgs a) {
   using S = TreeShape<HD, FMT, NT, RG, KG>;
   constexpr bool CODES = FMT != NCM_KV_BF16;
   constexpr int RB = S::kRowBytes, CPR = RB / 16, ROWS = S::kRows, NST = S::kStages;
@@ -284,16 +112,8 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
   const int gt = rg * 32 + lane;  // thread of the key group
   const uint32_t ring = smem_u32(smem) + kg * NST * S::kStageBytes;
   pdl_wait();
-  pdl_launch_dependents();
 
-  const long long total = units_before<ROWS>(a, a.batch.batch);
-  const long long lo = total * blockIdx.x / a.grid, hi = total * (blockIdx.x + 1) / a.grid;
-  if (blockIdx.x == 0 && warp == 0)
-    for (int b = lane; b < a.batch.batch; b += 32) load_seq(a, b, true);
-  if (lo >= hi) return;
-  long long inside;
-  int b = find_unit<ROWS>(a, lo, &inside);
-
+  Walk<ROWS> w(a, blockIdx.x, a.grid);
   auto group_sync = [&] {
     if constexpr (RG == 1)
       __syncwarp();
@@ -301,40 +121,26 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
       asm volatile("bar.sync %0, %1;" ::"r"(1 + kg), "n"(32 * RG) : "memory");
   };
 
-  for (long long at = lo; at < hi && b < a.batch.batch;) {
-    const Seq s = load_seq(a, b, false);
-    const int units = units_of(a, s);
-    const int tiles = tiles_of<ROWS>(a, s);
-    if (inside >= static_cast<long long>(units) * tiles * a.pools.kv_heads) {  // (empty sequences too)
-      ++b;
-      inside = 0;
-      continue;
-    }
-    const int item = static_cast<int>(inside / units), u0 = static_cast<int>(inside - static_cast<long long>(item) * units);
-    const int u1 = static_cast<int>(min(static_cast<long long>(units), u0 + (hi - at)));
-    const int kvh = item / tiles, row0 = (item - kvh * tiles) * ROWS;
-    const int ctx = s.len - s.n;
-    const int key0 = u0 * a.unit_keys, key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) * a.unit_keys));
-    const int live_rows = s.n * a.group - row0;  // rows of this tile that exist (may be more than ROWS)
+  while (w.next(a)) {
+    const Seq s = w.s;
+    const int kvh = w.kvh, row0 = w.row0, live_rows = w.live_rows, ctx = w.ctx, key0 = w.key0, key1 = w.key1;
 
     // ---- this key group's tiles: key0 + 32 (kg + KG i)
-    const int32_t* table = a.batch.page_table + b * a.batch.table_stride;
+    const int32_t* table = a.batch.page_table + w.b * a.batch.table_stride;
     const int ntiles = (key1 - key0 + kTile - 1) / kTile;
     const int mine = ntiles > kg ? (ntiles - kg + KG - 1) / KG : 0;
     const int page_mask = (1 << a.pools.page_shift) - 1;
-    // page of key (lane) of tile i, or -1
+    // page of key (lane) of tile i (asked for one tile ahead of its use); -1 behind the last key
     auto page_of = [&](int i) {
       const int key = key0 + kTile * (kg + KG * i) + lane;
-      if (i >= mine || key >= key1) return -1;
-      const int p = __ldg(table + (key >> a.pools.page_shift));
-      if (p < 0 || p >= a.pools.num_pages) {
-        atomicOr(a.err, kErrBadIndex);
-        return -1;
-      }
-      return p;
+      return i < mine && key < key1 ? __ldg(table + (key >> a.pools.page_shift)) : -1;
     };
     auto issue = [&](int i, int pages) {
       if (i < mine) {
+        if (pages < 0 || pages >= a.pools.num_pages) {
+          if (key0 + kTile * (kg + KG * i) + lane < key1) atomicOr(a.err, kErrBadIndex);
+          pages = -1;
+        }
         const int base = key0 + kTile * (kg + KG * i);
         const uint32_t st = ring + (i % NST) * S::kStageBytes;
         constexpr int PER = kTile * CPR / (32 * RG);
@@ -695,8 +501,8 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
         }
       }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == units;
-    float* part = a.part + (2ll * blockIdx.x + (u0 == 0 ? 1 : 0)) * ROWS * STR;
+    const bool whole = w.whole();
+    float* part = a.part + (2ll * blockIdx.x + (w.u0 == 0 ? 1 : 0)) * ROWS * STR;
     const int rows = min(ROWS, live_rows);
     for (int x = threadIdx.x; x < rows * (HD / 4); x += S::kThreads) {
       const int row = x / (HD / 4), d = (x % (HD / 4)) * 4;
@@ -735,108 +541,170 @@ __global__ void __launch_bounds__(32 * RG * KG) tree_attention_kernel(const Tree
       }
     }
     __syncthreads();
-    at += u1 - u0;
-    inside += u1 - u0;
   }
 }
 
 // Adds up the partial sums of one row of one item (blockIdx.x: sequence and kv
-// head, blockIdx.y: row of the sequence's rows). Four warps share the CTAs
-// that worked on the item; their sums are added in warp order.
+// head, blockIdx.y: row of the sequence's rows), in an order that the split
+// alone decides. An item of one long sequence may have a part from every CTA,
+// so the parts' maxima and sums are fetched by one thread each, and their
+// values by 128 / (HD / 4) groups of threads with four loads in flight.
+//
+// What the caller gave is read before the wait: the attention kernel lets this
+// one start only after its own wait, so the kernels in front of it are done.
+constexpr int kMaxParts = 2048;  // CTAs of the attention kernel at most
+
 template <int HD>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int ROWS) {
-  pdl_wait();
-  pdl_launch_dependents();
-  constexpr int DPL = HD / 32;
-  constexpr int STR = HD + 4;
-  __shared__ float sh[4][STR];
+  constexpr int STR = HD + 4, LPP = HD / 4, GROUPS = 128 / LPP;  // lanes of a part, parts at a time
+  __shared__ float weight[kMaxParts];
+  __shared__ float red[4][3];
+  __shared__ float4 vals[GROUPS][LPP];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / a.pools.kv_heads, kvh = blockIdx.x - b * a.pools.kv_heads;
   const Seq s = load_seq(a, b, false);
   const int row_all = blockIdx.y;
-  if (row_all >= s.n * a.group) return;
+  const bool exists = row_all < s.n * a.group;
   const int tile = row_all / ROWS, row = row_all - tile * ROWS;
-  auto tiles = [&](const Seq& q) { return (q.n * a.group + ROWS - 1) / ROWS; };
-  const int units = units_of(a, s);
-  long long before = 0, all = 0;
-  for (int i = lane; i < a.batch.batch; i += 32) {
-    const Seq q = load_seq(a, i, false);
-    const long long u = static_cast<long long>(tiles(q)) * a.pools.kv_heads * units_of(a, q);
-    all += u;
-    if (i < b) before += u;
+  int c0 = 0, c1 = 0;
+  long long all = 0;
+  if (exists) {
+    auto tiles = [&](const Seq& q) { return (q.n * a.group + ROWS - 1) / ROWS; };
+    const int units = units_of(a, s);
+    long long before = 0;
+    for (int i = lane; i < a.batch.batch; i += 32) {
+      const Seq q = load_seq(a, i, false);
+      const long long u = static_cast<long long>(tiles(q)) * a.pools.kv_heads * units_of(a, q);
+      all += u;
+      if (i < b) before += u;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units, x1 = x0 + units - 1;
+    c0 = static_cast<int>(((x0 + 1) * a.grid - 1) / all);
+    c1 = static_cast<int>(((x1 + 1) * a.grid - 1) / all);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (c0 == c1) return;  // one CTA had the whole item, and wrote its rows
+  const int n = c1 - c0 + 1;
+  const float* first = a.part + row * STR;
+  auto part_of = [&](int k) { return first + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * ROWS * STR; };
+  // a grid larger than the number of units has CTAs without any
+  auto empty = [&](int k) { return all < a.grid && all * (c0 + k) / a.grid == all * (c0 + k + 1) / a.grid; };
+  // ---- maxima, then the weights of the parts and the sum
+  float mm = kFirstMax, mv = kFirstMax;
+  for (int k = threadIdx.x; k < n; k += 128) {
+    if (empty(k)) continue;
+    const float4 h = *reinterpret_cast<const float4*>(part_of(k));
+    mm = fmaxf(mm, h.x);
+    mv = fmaxf(mv, h.z);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units, x1 = x0 + units - 1;
-  const int c0 = static_cast<int>(((x0 + 1) * a.grid - 1) / all), c1 = static_cast<int>(((x1 + 1) * a.grid - 1) / all);
-  if (c0 == c1) return;
-  float mm = kFirstMax, mv = kFirstMax, sum = 0.f, v[DPL];
-#pragma unroll
-  for (int d = 0; d < DPL; ++d) v[d] = 0.f;
-  auto add = [&](const float* src) {
-    const float top = fmaxf(mm, src[0]), topv = fmaxf(mv, src[2]);
-    sum = sum * ex2(mm - top) + src[1] * ex2(src[0] - top);
-    const float f = ex2(mv - topv), g = ex2(src[2] - topv);
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) v[d] = v[d] * f + src[4 + lane + 32 * d] * g;
-    mm = top;
-    mv = topv;
-  };
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    // (a grid larger than the number of units has CTAs without any between c0 and c1)
-    if (all * c / a.grid == all * (c + 1) / a.grid) continue;
-    add(a.part + ((2ll * c + (c == c0 ? 1 : 0)) * ROWS + row) * STR);
+    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
   }
   if (lane == 0) {
-    sh[warp][0] = mm;
-    sh[warp][1] = sum;
-    sh[warp][2] = mv;
+    red[warp][0] = mm;
+    red[warp][1] = mv;
+  }
+  __syncthreads();
+  mm = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  mv = fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1]));
+  float sum = 0.f;
+  for (int k = threadIdx.x; k < n; k += 128) {
+    float w = 0.f;
+    if (!empty(k)) {
+      const float4 h = *reinterpret_cast<const float4*>(part_of(k));
+      w = ex2(h.z - mv);
+      sum = fmaf(h.y, ex2(h.x - mm), sum);
+    }
+    weight[k] = w;
   }
 #pragma unroll
-  for (int d = 0; d < DPL; ++d) sh[warp][4 + lane + 32 * d] = v[d];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp][2] = sum;
   __syncthreads();
-  if (warp != 0) return;
-  for (int w = 1; w < 4; ++w) add(sh[w]);
+  sum = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
+  // ---- values
+  const int g = threadIdx.x / LPP, d = threadIdx.x % LPP;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = g; k0 < n; k0 += 4 * GROUPS) {
+    float4 y[4];
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + i * GROUPS;
+      w[i] = k < n ? weight[k] : 0.f;
+      y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < n && !empty(k)) y[i] = *reinterpret_cast<const float4*>(part_of(k) + 4 + 4 * d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v.x = fmaf(y[i].x, w[i], v.x);
+      v.y = fmaf(y[i].y, w[i], v.y);
+      v.z = fmaf(y[i].z, w[i], v.z);
+      v.w = fmaf(y[i].w, w[i], v.w);
+    }
+  }
+  vals[g][d] = v;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) {
+    const float4 y = vals[k][d];
+    v.x += y.x;
+    v.y += y.y;
+    v.z += y.z;
+    v.w += y.w;
+  }
   const int i = row_all / a.group, head = kvh * a.group + row_all - i * a.group;
   const long long t = s.first + static_cast<long long>(i);
-  const float f = out_factor(sum, mv - mm), g = half_power(mv - mm);
-#pragma unroll
-  for (int d = 0; d < DPL; ++d)
-    a.out[t * a.out_stride + head * HD + lane + 32 * d] = static_cast<uint16_t>(pack_rn_bf16x2(v[d] * f * g, 0.f));
-  if (lane == 0 && a.lse != nullptr) a.lse[t * a.heads + head] = lse_of(mm, sum);
+  const float f = out_factor(sum, mv - mm), h = half_power(mv - mm);
+  *reinterpret_cast<uint2*>(a.out + t * a.out_stride + head * HD + 4 * d) =
+      make_uint2(pack_rn_bf16x2(v.x * f * h, v.y * f * h), pack_rn_bf16x2(v.z * f * h, v.w * f * h));
+  if (d == 0 && a.lse != nullptr) a.lse[t * a.heads + head] = lse_of(mm, sum);
 }
 
-using TreeKernel = void (*)(const TreeArgs);
-struct Variant {
-  TreeKernel kernel;
-  int rows, threads, smem;
-};
+using Variant = TreeTcVariant;
 template <int HD, int FMT, int NT, int RG, int KG>
 constexpr Variant variant() {
   using S = TreeShape<HD, FMT, NT, RG, KG>;
   return Variant{tree_attention_kernel<HD, FMT, NT, RG, KG>, S::kRows, S::kThreads, S::kSmem};
 }
 
-// By the rows of one kv head: 8, 16, 32, 64 or 128 rows a tile. Few rows take
-// the keys four groups at a time, many share each tile among four row groups.
-constexpr int kSizes = 5;
+// By the rows of one kv head: 8, 16, 32 or 64 rows a tile. Few rows take the
+// keys four groups at a time, more share each tile among row groups.
+constexpr int kSizes = 4;
 template <int FMT>
 struct Variants {
   static constexpr Variant hd64[kSizes] = {variant<64, FMT, 1, 1, 4>(), variant<64, FMT, 2, 1, 4>(), variant<64, FMT, 4, 1, 4>(),
-                                           variant<64, FMT, 4, 2, 2>(), variant<64, FMT, 4, 4, 1>()};
+                                           variant<64, FMT, 4, 2, 2>()};
   static constexpr Variant hd128[kSizes] = {variant<128, FMT, 1, 1, 4>(), variant<128, FMT, 2, 1, 4>(), variant<128, FMT, 2, 2, 2>(),
-                                            variant<128, FMT, 2, 4, 1>(), variant<128, FMT, 2, 4, 1>()};
+                                            variant<128, FMT, 2, 4, 1>()};
 };
 
-const Variant& pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
+// Rows of one kv head that stay with the mma.sync kernel. More go to the tcgen05
+// kernel, whose tiles have 128 rows. us of both, mma.sync / tcgen05 (eight
+// sequences of 1 to 16 thousand tokens, 8 kv heads): 64 rows, bf16: 56 / 79 at
+// head_dim 64, 81 / 107 at 128, int8: 66 / 77 and 92 / 111; 128 rows, bf16: 100 /
+// 89 and 160 / 125, int8: 113 / 92 and 177 / 126; 256 rows: 187 / 131, 300 / 227, 207 /
+// 148 and 326 / 219.
+constexpr int64_t kFewRows = 64;
+Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
   const bool wide = c->head_dim == 128;
+  if (rows > kFewRows) {
+    *index = 3 * 2 * kSizes + (c->format * 2 + wide) * 2 + (rows > 128);
+    return tree_tc_variant(c->format, c->head_dim, rows);
+  }
   const Variant* v = c->format == NCM_KV_BF16   ? (wide ? Variants<NCM_KV_BF16>::hd128 : Variants<NCM_KV_BF16>::hd64)
                      : c->format == NCM_KV_INT8 ? (wide ? Variants<NCM_KV_INT8>::hd128 : Variants<NCM_KV_INT8>::hd64)
                                                 : (wide ? Variants<NCM_KV_E4M3>::hd128 : Variants<NCM_KV_E4M3>::hd64);
-  const int i = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 3 : 4;
+  const int i = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
   *index = (c->format * 2 + wide) * kSizes + i;
   return v[i];
 }
@@ -865,8 +733,8 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
     return ncm_fail(NCM_EINVAL, "%s: too many sequences", what);
   int index = 0;
   p->v = pick(cache, static_cast<int64_t>(max_nodes) * (heads / cache->kv_heads), &index);
-  static std::atomic<int> resident[3 * 2 * kSizes];  // CTAs of a variant on one SM
-  static DeviceFlags ready[3 * 2 * kSizes];
+  static std::atomic<int> resident[3 * 2 * (kSizes + 2)];  // CTAs of a variant on one SM
+  static DeviceFlags ready[3 * 2 * (kSizes + 2)];
   if (!ready[index].test(ctx->device)) {
     int n = 0;
     NCM_CUDA_TRY(cudaFuncSetAttribute(p->v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p->v.smem));
@@ -877,7 +745,7 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
   const int64_t cap = static_cast<int64_t>(batch->table_width) * cache->page_size;
   p->merge = cap > kWholeKeys;
   p->unit_keys = p->merge ? kUnitKeys : static_cast<int>(kWholeKeys);
-  p->grid = ctx->num_sms * resident[index].load();
+  p->grid = std::min(kMaxParts, ctx->num_sms * resident[index].load());
   p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
   return NCM_OK;
 }

@@ -1,0 +1,243 @@
+// What the two attention kernels over the paged cache and their merge share:
+// arguments, the split of the work, masks and the last steps of a row.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace ncm {
+
+constexpr float kFirstMax = -1e30f;
+constexpr float kSlack = 8.f;  // scores may pass the running maximum by 2^8
+
+struct TreeArgs {
+  KvPools pools;
+  KvBatch batch;
+  const uint16_t* q;
+  long long q_stride;
+  const uint32_t* mask;
+  int mask_words;
+  int heads, group, max_nodes;
+  float scale_log2;
+  uint16_t* out;
+  long long out_stride;
+  float* lse;
+  float* part;  // [2 * grid][ROWS][4 + HD]: m, sum of p, m', -, values
+  int unit_keys;
+  int grid;  // CTAs of the attention kernel
+  int* err;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// 16 (4) bytes from global to shared memory, zeros where !live.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_rn_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Four codes as two pairs of f16, exactly: bytes (0, 1) and (2, 3).
+template <int FMT>
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t* lo, uint32_t* hi) {
+  if constexpr (FMT == NCM_KV_INT8) {
+    w ^= 0x80808080u;  // 128 + code; 0x6400 | b is 1024 + b
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*lo) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*hi) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(*lo), "=r"(*hi)
+        : "r"(w));
+  }
+}
+// The same of bytes (0, 2) and (1, 3).
+template <int FMT>
+__device__ __forceinline__ void code_pairs_strided(uint32_t w, uint32_t* even, uint32_t* odd) {
+  if constexpr (FMT == NCM_KV_INT8) {
+    w ^= 0x80808080u;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*even) : "r"(__byte_perm(w, 0x64646464u, 0x4240)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*odd) : "r"(__byte_perm(w, 0x64646464u, 0x4341)), "r"(0x64806480u));
+  } else {
+    code_pairs<FMT>(__byte_perm(w, 0u, 0x3120), even, odd);
+  }
+}
+
+// What one sequence contributes: its nodes (0 where its numbers do not fit), keys and units.
+struct Seq {
+  int first, n, len;
+};
+__device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, bool report) {
+  Seq s;
+  s.first = __ldg(a.batch.token_start + b);
+  s.n = __ldg(a.batch.token_start + b + 1) - s.first;
+  s.len = __ldg(a.batch.kv_lens + b);
+  const bool bad = s.first < 0 || s.n < 0 || s.n > a.max_nodes || s.len < s.n ||
+                   static_cast<long long>(s.first) + s.n > a.batch.rows ||
+                   s.len > (static_cast<long long>(a.batch.table_width) << a.pools.page_shift);
+  if (bad) {
+    if (report) atomicOr(a.err, kErrBadIndex);
+    s.n = s.len = 0;
+  }
+  return s;
+}
+
+template <int ROWS>
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) {
+  return (s.n * a.group + ROWS - 1) / ROWS;
+}
+__device__ __forceinline__ int units_of(const TreeArgs& a, const Seq& s) { return (s.len + a.unit_keys - 1) / a.unit_keys; }
+
+// Units in front of sequence `upto` (whole warps; every lane gets the sum).
+template <int ROWS>
+__device__ __forceinline__ long long units_before(const TreeArgs& a, int upto) {
+  long long sum = 0;
+  for (int b = threadIdx.x & 31; b < upto; b += 32) {
+    const Seq s = load_seq(a, b, false);
+    sum += static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// The sequence that holds unit x < total, and the unit's place in it.
+template <int ROWS>
+__device__ __forceinline__ int find_unit(const TreeArgs& a, long long x, long long* inside) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
+    long long u = 0;
+    if (b0 + lane < a.batch.batch) {
+      const Seq s = load_seq(a, b0 + lane, false);
+      u = static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
+    }
+    long long before = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    const long long all = __shfl_sync(0xffffffffu, before, 31);
+    before -= u;
+    if (x < all) {
+      const unsigned hit = __ballot_sync(0xffffffffu, x >= before && x < before + u);
+      const int who = __ffs(hit) - 1;
+      *inside = x - __shfl_sync(0xffffffffu, before, who);
+      return b0 + who;
+    }
+    x -= all;
+  }
+  *inside = 0;
+  return a.batch.batch;
+}
+
+// Bits [j0, j0 + 32) of a node's mask row (bits in front of 0 are ones, behind the row zeros).
+__device__ __forceinline__ uint32_t mask_window(const uint32_t* row, int words, int j0) {
+  if (j0 <= -32) return 0xFFFFFFFFu;
+  if (j0 < 0) {
+    const uint32_t w = words > 0 ? __ldg(row) : 0u;
+    return (w << -j0) | ((1u << -j0) - 1u);
+  }
+  const int i = j0 >> 5;
+  const uint32_t lo = i < words ? __ldg(row + i) : 0u, hi = i + 1 < words ? __ldg(row + i + 1) : 0u;
+  return __funnelshift_r(lo, hi, j0 & 31);
+}
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+
+// The segments of one CTA, in order: runs of consecutive units of one item
+// (sequence, kv head, tile of ROWS rows). Every thread walks the same ones.
+template <int ROWS>
+struct Walk {
+  long long at, hi, inside;
+  int b;
+  Seq s;
+  int units, u0, u1;
+  int kvh, row0, live_rows;  // (live_rows: rows of the item from row0 on; may be more than ROWS)
+  int ctx, key0, key1;
+
+  // Whole warps; block 0 of `blocks` reports sequences that do not fit.
+  __device__ __forceinline__ Walk(const TreeArgs& a, int block, int blocks) {
+    const long long total = units_before<ROWS>(a, a.batch.batch);
+    at = total * block / blocks;
+    hi = total * (block + 1) / blocks;
+    if (block == 0 && threadIdx.x < 32)
+      for (int i = threadIdx.x; i < a.batch.batch; i += 32) load_seq(a, i, true);
+    inside = 0;
+    b = at < hi ? find_unit<ROWS>(a, at, &inside) : a.batch.batch;
+    u0 = u1 = 0;
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a) {
+    at += u1 - u0;
+    inside += u1 - u0;
+    u0 = u1 = 0;
+    while (at < hi && b < a.batch.batch) {
+      s = load_seq(a, b, false);
+      units = units_of(a, s);
+      const int tiles = tiles_of<ROWS>(a, s);
+      if (inside >= static_cast<long long>(units) * tiles * a.pools.kv_heads) {  // (empty sequences too)
+        ++b;
+        inside = 0;
+        continue;
+      }
+      const int item = static_cast<int>(inside / units);
+      u0 = static_cast<int>(inside - static_cast<long long>(item) * units);
+      u1 = static_cast<int>(min(static_cast<long long>(units), u0 + (hi - at)));
+      kvh = item / tiles;
+      row0 = (item - kvh * tiles) * ROWS;
+      live_rows = s.n * a.group - row0;
+      ctx = s.len - s.n;
+      key0 = u0 * a.unit_keys;
+      key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) * a.unit_keys));
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == units; }
+};
+
+// 2^(d / 2), twice: the values' sums are brought from their maximum to the
+// scores' by 2^d, which alone may pass f32's range.
+__device__ __forceinline__ float half_power(float d) { return ex2(0.5f * d); }
+// half_power(d) / sum; 0 for a row that saw nothing.
+__device__ __forceinline__ float out_factor(float sum, float d) { return sum == 0.f ? 0.f : __fdiv_rn(half_power(d), sum); }
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  return sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
+}
+
+// The tcgen05 kernel (tree_attention_tc.cu): its launch, and what the plan needs of it.
+struct TreeTcVariant {
+  void (*kernel)(const TreeArgs);
+  int rows, threads, smem;
+};
+TreeTcVariant tree_tc_variant(int format, int head_dim, int64_t rows);
+
+}  // namespace ncm

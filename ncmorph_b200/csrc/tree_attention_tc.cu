@@ -1,0 +1,733 @@
+// Attention of many drafted tokens over the paged cache: the same operator, split
+// and partial sums as tree_attention.cu, for items whose query rows fill more of a
+// 128-row tensor-core tile (rows: nodes x the query heads of one kv head). Per key
+// tile of 64:
+//   S = Q K^T    tcgen05.mma M=128 N=64 K=head_dim, f32 in tensor memory (two buffers)
+//   softmax      one thread per row; P (bf16) into a 128-byte-swizzled tile (two buffers)
+//   O += P V     tcgen05.mma M=128 N=head_dim K=64, accumulated in tensor memory
+// Two groups of four softmax warps work side by side, because one row's tile is
+// a chain of waits (scores, maximum, exponentials, hand-over) three times as long as
+// its exponentials: with up to 128 rows they take every other key tile and add
+// their sums up at the end, with more (head_dim 64) each has 128 rows of its own.
+// Two more warps issue the groups' products; eight load. Every key
+// and value is fetched and, for int8 and e4m3, turned into bf16 (exactly) once per CTA,
+// whatever the number of rows; in the mma.sync kernel each 8 to 32 rows do that again.
+// A key's scale multiplies its scores, a value's scale its probability. V is
+// taken as it lies in the cache, head_dim contiguous: the second product's B
+// operand is MN-major.
+//
+// Bound: with more than about 64 rows the exponentials (16 a clock and SM: 128
+// rows of 64 keys take 512 clocks, the two products 256 at head_dim 64), with fewer
+// the cache's bytes. The maximum moves only past 2^8 (kSlack), as in the other
+// kernel; then O is rescaled in tensor memory.
+//
+// A value row of a new token that holds a NaN or an infinity and is hidden from some rows
+// must not reach them as 0 * NaN: the loaders put zeros in the place of such values, and
+// rows that see them add them at the end.
+#include "tree_attention.cuh"
+
+namespace ncm {
+namespace {
+
+constexpr int kLoadWarps = 4;  // of a group
+constexpr int kLoadThreads = 32 * kLoadWarps;
+
+struct TcBars {
+  uint64_t q_full;
+  uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
+  uint64_t s_full[2][2], s_free[2][2];  // [group][buffer]
+  uint64_t p_full[2][2], pv_done[2][2];
+  uint64_t sums_full[4], cols_full[4][2], cols_free[4][2];  // [warp pair] the second group's sums, and 32 columns of its values
+  uint64_t drain[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  float2 sums[128];  // the second group's maxima and sums
+  int odd_values;  // a loader met a value that is not finite in a tile of new tokens
+};
+constexpr int kBarBytes = 2048;
+static_assert(sizeof(TcBars) <= kBarBytes, "barriers");
+
+// SPLITQ: the groups have 128 rows each; otherwise the same 128 rows and every other tile.
+template <int HD, int FMT, bool SPLITQ>
+struct TcShape {
+  static_assert(!SPLITQ || HD == 64, "256 rows fit with head_dim 64 only");
+  static constexpr bool kCodes = FMT != NCM_KV_BF16;
+  static constexpr int kQTiles = SPLITQ ? 2 : 1;
+  static constexpr int kRows = 128 * kQTiles;
+  // Two groups of loaders take every other tile, so that one's waits and conversion run
+  // beside the other's. A bf16 tile that 256 rows share lasts long enough for one
+  // group, which leaves 128 registers a thread.
+  static constexpr int kLoadGroups = SPLITQ && !kCodes ? 1 : 2;
+  static constexpr int kThreads = 32 * (8 + 2 + kLoadGroups * kLoadWarps);
+  static constexpr int kRowBytes = HD * (kCodes ? 1 : 2);
+  // Keys of a tile: what a row waits for per tile is the same for 64 keys and for
+  // 128, but 128 of 128-wide heads do not fit beside the rest.
+  static constexpr int kBK = HD == 64 ? 128 : 64;
+  static constexpr int kSBufs = 128 / kBK;  // buffers of S
+  // Tiles in bf16; codes: raw tiles in flight in front of them (of both groups of
+  // loaders), in shared memory, or (head_dim 128, where that is full) one a group in registers.
+  static constexpr int kStages = kCodes && HD == 64 ? 2 : 4;
+  static constexpr bool kInRegs = kCodes && HD == 128;
+  static constexpr int kRaw = !kCodes || kInRegs ? 0 : 2;
+  static constexpr int kPBufs = kInRegs ? 1 : kSBufs;  // buffers of P, of 128 rows x kBK keys
+  static constexpr int kPBytes = 256 * kBK;
+  // tiles that a group of loaders has asked for before it waits for the first of them
+  static constexpr int kAhead = kLoadGroups == 1 ? 2 : 1;
+  // (a stage's uses all belong to one group of loaders, and to one of softmax warps
+  // where those take every other tile: each waits for its own earlier use)
+  static_assert(kStages % 2 == 0, "stages per group");
+  // Slots of the scales: a K stage is free again when its S is issued, up to two tiles of
+  // its group ahead of the softmax that still reads an earlier tile's scales.
+  static constexpr int kScaleSlots = kStages + 8;
+  static constexpr int kBlocks = HD / 64;  // 64-dim columns of a tile
+  static constexpr int kQ = 0;
+  static constexpr int kP = kQ + kQTiles * kBlocks * 16384;  // [group][buffer]
+  static constexpr int kK = kP + 2 * kPBufs * kPBytes;
+  static constexpr int kBlock = 128 * kBK;  // bytes of 64 dims of a K or V tile
+  static constexpr int kV = kK + kStages * kBlocks * kBlock;
+  static constexpr int kRawAt = kV + kStages * kBlocks * kBlock;
+  static constexpr int kScale = kRawAt + kRaw * 2 * kBK * kRowBytes;  // [slot][K, V][kBK] f32
+  static constexpr bool kRawScales = kCodes && !kInRegs;
+  static constexpr int kRawScale = kScale + (kCodes ? kScaleSlots * 2 * kBK * 4 : 0);  // [raw][K, V][kBK] f32
+  static constexpr int kBars = kRawScale + (kRawScales ? kRaw * 2 * kBK * 4 : 0);
+  static constexpr int kSmem = kBars + kBarBytes + 1024;  // (1024: the base is aligned up)
+  static constexpr uint32_t kTmemCols = 512;  // S: 2 x 2 x 64, O: 2 x head_dim
+  static_assert(kSmem <= 232448, "shared memory of the tcgen05 attention");
+};
+
+// Instruction descriptor: bf16 operands, f32 sums, M = 128; B MN-major where `mn`.
+__device__ constexpr uint32_t tc_idesc(int n, bool mn) { return idesc_bf16_f32(128, n) | (mn ? 1u << 16 : 0u); }
+
+// Descriptor of an MN-major bf16 tile with 128-byte swizzling: rows (the
+// contracted index) of 64 elements, 8-row groups 1024 bytes apart, further
+// 64-element columns `column` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t column) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | static_cast<uint64_t>(column >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+// Bytes I and J of w as two bf16 values, exactly. int8: 128 + (low seven bits) minus
+// 128 or 256, by the sign bit. e4m3: the code's exponent and mantissa moved into
+// bf16's fields are the value times 2^-120 (subnormal codes included).
+template <int FMT>
+__device__ __forceinline__ uint32_t code_pair_bf16(uint32_t w, uint32_t hi) {
+  uint32_t r;
+  if constexpr (FMT == NCM_KV_INT8) {
+    const uint32_t x = __byte_perm(w, 0x43434343u, hi ? 0x4342 : 0x4140);
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0x437F437Fu), "r"(x & 0x43804380u));
+  } else {
+    const uint32_t x = __byte_perm(w, 0u, hi ? 0x3424 : 0x1404);
+    const uint32_t y = ((x & 0x7F007F00u) >> 4) | (x & 0x80008000u);
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(y), "r"(0x7B807B80u));  // 2^120
+  }
+  return r;
+}
+
+// mbar_wait for a kernel whose warps mostly wait: between tries the thread is
+// suspended until the phase completes (or 20 us pass), and leaves the issue slots to the others.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t since = 0;
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    const uint64_t now = globaltimer_ns();
+    if (since == 0) since = now;
+    if (*abort || now - since > kWaitLimitNs) return false;
+  }
+}
+
+template <int HD, int FMT, bool SPLITQ>
+__global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_attention_tc_kernel(const TreeArgs a) {
+  using S = TcShape<HD, FMT, SPLITQ>;
+  constexpr bool CODES = S::kCodes;
+  constexpr int BK = S::kBK, RB = S::kRowBytes, CPR = RB / 16, NS = S::kStages, LG = S::kLoadGroups, NB = S::kBlocks, ROWS = S::kRows;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&B.q_full, 4 * S::kQTiles);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&B.k_full[i], kLoadWarps);
+      mbar_init(&B.v_full[i], kLoadWarps);
+      mbar_init(&B.k_empty[i], S::kQTiles);
+      mbar_init(&B.v_empty[i], S::kQTiles);
+    }
+    for (int g = 0; g < 2; ++g)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&B.s_full[g][i], 1);
+        mbar_init(&B.s_free[g][i], 4);
+        mbar_init(&B.p_full[g][i], 4);
+        mbar_init(&B.pv_done[g][i], 1);
+      }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&B.sums_full[i], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&B.cols_full[i][x], 1);
+        mbar_init(&B.cols_free[i][x], 1);
+      }
+    }
+    mbar_init(&B.drain[0], 1);
+    mbar_init(&B.drain[1], 1);
+    B.abort_flag = 0;
+    B.odd_values = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&B.tmem_base, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = B.tmem_base;  // S of group g: columns 128 g on; O of group g: 256 + HD g
+  volatile int* abort_flag = &B.abort_flag;
+  auto fail = [&] {
+    *abort_flag = 1;
+    atomicOr(a.err, kErrWaitTimeout);
+  };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {  // one lane waits for its warp
+    int done = 1;
+    if (lane == 0) done = tc_wait(bar, parity, abort_flag);
+    return __shfl_sync(0xffffffffu, done, 0) != 0;
+  };
+  Walk<ROWS> w(a, blockIdx.x, a.grid);
+  uint32_t number = 0;  // of the segment's first tile: they are numbered over all segments
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax
+    const int g = warp >> 2, qt = SPLITQ ? g : 0, row = (warp & 3) * 32 + lane;
+    constexpr int STEP = SPLITQ ? 1 : 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t obase = tmem + lanes + 256 + g * HD;
+    uint32_t j = 0, segment = 0, rounds = 0;  // tiles, segments and sums handed over so far
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {  // (uniform over the warp)
+      ok = warp_wait(bar, parity);
+      return ok;
+    };
+    for (; ok && w.next(a); ++segment) {
+      const int live = w.live_rows - qt * 128;  // rows of this query tile
+      const int ntiles = (w.key1 - w.key0 + BK - 1) / BK;
+      const uint32_t n0 = number;
+      number += ntiles;
+      const int row_all = w.row0 + qt * 128 + row;
+      const bool exists = row < live;
+      const int node = exists ? row_all / a.group : -1;
+      const int head = w.kvh * a.group + (exists ? row_all - node * a.group : 0);
+      const long long token = w.s.first + static_cast<long long>(exists ? node : 0);
+      if (SPLITQ || g == 0) {
+        if (exists) {
+          const uint16_t* src = a.q + token * a.q_stride + head * HD;
+          uint8_t* dst = smem + S::kQ + qt * NB * 16384 + row * 128;
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c)
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = *reinterpret_cast<const uint4*>(src + 8 * c);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.q_full);
+      }
+      if (SPLITQ && live <= 0) {  // nothing in this query tile: its products are not issued
+        // (not ahead of the others: a second arrival must not count for this segment)
+        if (!wait(&B.q_full, segment & 1u)) break;
+        continue;
+      }
+      const bool busy = (warp & 3) * 32 < live;  // (a warp without rows only keeps the barriers going)
+      float m = kFirstMax, l = 0.f;
+      bool any = false;  // O holds something
+      for (int t = SPLITQ ? 0 : g; t < ntiles; t += STEP, ++j) {
+        const int buf = j & 1;
+        if (!wait(&B.s_full[g][buf], (j >> 1) & 1u)) break;
+        if (busy) {
+          tc_fence_after();
+          const uint32_t sbase = tmem + lanes + 128 * g + (j % S::kSBufs) * BK;
+          const float4* scales = reinterpret_cast<const float4*>(smem + S::kScale + ((n0 + t) % S::kScaleSlots) * 2 * BK * 4);
+          const int base = w.key0 + t * BK;
+          const bool partly = base + BK > min(w.ctx, w.key1);
+          // P's buffer is free once the product that read it last is done
+          constexpr uint32_t PB = S::kPBufs;
+          if (j >= PB && !wait(&B.pv_done[g][(j - PB) & 1], ((j - PB) >> 1) & 1u)) break;
+          uint8_t* prow = smem + S::kP + (PB * g + j % PB) * S::kPBytes + row * 128;
+          // Scores: raw where they take the scale with the exponent (bf16 cache,
+          // positive scale), otherwise in units of log2; -inf where hidden.
+          const bool late = !CODES && a.scale_log2 > 0.f;
+          const float scale = late ? a.scale_log2 : 1.f;
+          // 32 keys at a time, so that a row's scores fit beside the rest in 96
+          // registers. The loop stays rolled: the roles' code together must not
+          // outgrow the instruction cache.
+#pragma unroll 1
+          for (int h = 0; h < BK / 32; ++h) {
+            uint32_t raw[32];
+            float* sc = reinterpret_cast<float*>(raw);
+            tmem_ld_x32(sbase + 32 * h, raw);
+            tmem_wait_ld();
+            if (h == BK / 32 - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
+            }
+            if (!late) {
+              const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const unsigned long long f = CODES ? f2_mul(reinterpret_cast<const unsigned long long*>(scales)[16 * h + i], up) : up;
+                f2_unpack(f2_mul(f2_pack(sc[2 * i], sc[2 * i + 1]), f), sc[2 * i], sc[2 * i + 1]);
+              }
+            }
+            uint32_t seen = 0xFFFFFFFFu;
+            if (partly) {
+              const int k0 = base + 32 * h;
+              seen = !exists ? 0u
+                             : first_bits(w.key1 - k0) & (a.mask == nullptr
+                                                              ? first_bits(w.ctx + node - k0 + 1)
+                                                              : mask_window(a.mask + token * a.mask_words, a.mask_words, k0 - w.ctx));
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((seen >> i) & 1u)) sc[i] = -INFINITY;
+            }
+            float x4[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+            for (int i = 4; i < 28; i += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], fmaxf(sc[i + e], sc[i + 4 + e]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], sc[28 + e]);
+            const float top = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * scale;
+            // The maximum only takes whole values, so that what it moves is multiplied by powers of two.
+            const bool move = exists && top > m + kSlack;
+            if (__any_sync(0xffffffffu, move)) {
+              const float to = move ? ceilf(top) : m;
+              const float f = ex2(m - to);
+              m = to;
+              l *= f;
+              if (any) {  // O holds the tiles before this one: wait for the last of them
+                if (!wait(&B.pv_done[g][buf ^ 1], ((j - 1) >> 1) & 1u)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 16) {
+                  uint32_t o[16];
+                  tmem_ld_x16(obase + d, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st_x16(obase + d, o);
+                }
+                tmem_wait_st();
+              }
+              // and the probabilities in front of these
+#pragma unroll 1
+              for (int c = 0; c < 4 * h; ++c) {
+                uint4* q = reinterpret_cast<uint4*>(prow + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4));
+                uint32_t e[4] = {q->x, q->y, q->z, q->w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = pack_rn_bf16x2(bf16lo(e[i]) * f, bf16hi(e[i]) * f);
+                *q = make_uint4(e[0], e[1], e[2], e[3]);
+              }
+            }
+            unsigned long long sum = f2_pack(0.f, 0.f);
+            const unsigned long long scale2 = f2_pack(scale, scale), minus_m = f2_pack(-m, -m);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = 8 * c + 2 * i;
+                float p0, p1;
+                f2_unpack(f2_fma(f2_pack(sc[k], sc[k + 1]), scale2, minus_m), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                sum = f2_add(sum, f2_pack(p0, p1));
+                if constexpr (CODES) {
+                  f2_unpack(f2_mul(f2_pack(p0, p1), reinterpret_cast<const unsigned long long*>(scales)[BK / 2 + 16 * h + k / 2]), p0, p1);
+                  if (partly) {  // (a hidden key's scale may be NaN)
+                    if (!((seen >> k) & 1u)) p0 = 0.f;
+                    if (!((seen >> (k + 1)) & 1u)) p1 = 0.f;
+                  }
+                }
+                e[i] = pack_rn_bf16x2(p0, p1);
+              }
+              *reinterpret_cast<uint4*>(prow + (h >> 1) * 16384 + (((4 * (h & 1) + c) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+            float s0, s1;
+            f2_unpack(sum, s0, s1);
+            l += s0 + s1;
+          }
+          if (!ok) break;
+        } else {
+          if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
+        }
+        any = true;
+        tc_fence_before();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.p_full[g][buf]);
+      }
+      if (ok && any) wait(&B.pv_done[g][(j - 1) & 1], ((j - 1) >> 1) & 1u);
+      if (!ok) break;
+      if (!busy) continue;
+      tc_fence_after();
+      // ---- this row's sums: out, or its part of them; the second group's go to the
+      // first through its own P buffers, [32 columns][128 rows] at a time, in XB buffers
+      const bool whole = w.whole();
+      const bool odd = !CODES && *const_cast<volatile int*>(&B.odd_values) != 0;
+      constexpr uint32_t XB = S::kPBufs * S::kPBytes / 16384;
+      float f0 = 1.f, f1 = 0.f;  // weights of the groups' values
+      if constexpr (!SPLITQ) {
+        if (g == 1) {
+          B.sums[row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.sums_full[warp & 3]);
+        } else {
+          if (!wait(&B.sums_full[warp & 3], (rounds / (HD / 32)) & 1u)) break;
+          const float2 other = B.sums[row];
+          const float to = fmaxf(m, other.x);
+          f0 = ex2(m - to);
+          f1 = ex2(other.x - to);
+          l = l * f0 + other.y * f1;
+          m = to;
+        }
+      }
+      float* part = a.part + ((2ll * blockIdx.x + (w.u0 == 0 ? 1 : 0)) * ROWS + qt * 128 + row) * (HD + 4);
+      uint16_t* out = a.out + token * a.out_stride + head * HD;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 32, ++rounds) {
+        uint32_t raw[32];
+        float* o = reinterpret_cast<float*>(raw);
+        if (any) {
+          tmem_ld_x32(obase + d, raw);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if constexpr (!SPLITQ) {
+          const uint32_t x = rounds % XB, parity = (rounds / XB) & 1u;
+          float* xch = reinterpret_cast<float*>(smem + S::kP + S::kPBufs * S::kPBytes + x * 16384) + row;
+          if (g == 1) {
+            if (!wait(&B.cols_free[warp & 3][x], parity ^ 1u)) break;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) xch[i * 128] = o[i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.cols_full[warp & 3][x]);
+            continue;
+          }
+          if (!wait(&B.cols_full[warp & 3][x], parity)) break;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + xch[i * 128] * f1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.cols_free[warp & 3][x]);
+        }
+        if (!exists) continue;
+        if (odd) {
+          // (the keys of the tiles with new tokens)
+          for (int k = w.key0 + (max(w.ctx - w.key0, 0) & ~(BK - 1)); k < w.key1; ++k) {
+            const int n2 = k - w.ctx;
+            if (!(a.mask == nullptr ? n2 <= node : (mask_window(a.mask + token * a.mask_words, a.mask_words, n2) & 1u) != 0u)) continue;
+            const int page = __ldg(a.batch.page_table + w.b * a.batch.table_stride + (k >> a.pools.page_shift));
+            if (page < 0 || page >= a.pools.num_pages) continue;
+            const uint16_t* v = static_cast<const uint16_t*>(a.pools.v) +
+                                kv_slot(a.pools, page, w.kvh, k & ((1 << a.pools.page_shift) - 1)) * HD + d;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((v[i] & 0x7F80u) == 0x7F80u) o[i] += bf16_to_f32(v[i]);
+          }
+        }
+        if (whole) {
+          const float f = out_factor(l, 0.f);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(out + d + i) =
+                make_uint4(pack_rn_bf16x2(o[i] * f, o[i + 1] * f), pack_rn_bf16x2(o[i + 2] * f, o[i + 3] * f),
+                           pack_rn_bf16x2(o[i + 4] * f, o[i + 5] * f), pack_rn_bf16x2(o[i + 6] * f, o[i + 7] * f));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part + 4 + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (!ok) break;
+      if (exists && (SPLITQ || g == 0)) {
+        if (!whole)
+          *reinterpret_cast<float4*>(part) = make_float4(m, l, m, 0.f);
+        else if (a.lse != nullptr)
+          a.lse[token * a.heads + head] = lse_of(m, l);
+      }
+      // the last columns must be taken before the second group's P buffers are written
+      // again (which also keeps the pair within one segment: sums has one place)
+      if (!SPLITQ && g == 1) {
+#pragma unroll
+        for (uint32_t x = 0; x < XB; ++x)
+          if (!wait(&B.cols_free[warp & 3][x], ((rounds / XB) & 1u) ^ 1u)) break;
+        if (!ok) break;
+      }
+      tc_fence_before();
+    }
+    if (!ok) fail();
+  } else if (warp < 10) {
+    // ------------------------------------------- the products of one group each
+    if (lane == 0) {
+      const int g = warp - 8;
+      constexpr uint32_t STEP = SPLITQ ? 1 : 2;
+      const uint32_t id_s = tc_idesc(BK, false), id_o = tc_idesc(HD, true);
+      const uint64_t dq = smem_desc_k_sw128(smem_u32(smem + S::kQ)) + (SPLITQ ? g * NB * 1024 : 0);
+      const uint64_t dk = smem_desc_k_sw128(smem_u32(smem + S::kK));
+      const uint64_t dp = smem_desc_k_sw128(smem_u32(smem + S::kP)) + g * (S::kPBufs * S::kPBytes / 16);
+      const uint64_t dv = smem_desc_mn_sw128(smem_u32(smem + S::kV), S::kBlock);
+      const uint32_t ts = tmem + 128 * g, to = tmem + 256 + g * HD;
+      uint32_t js = 0, jo = 0, segment = 0;  // products issued, of each kind
+      bool ok = true;
+      auto issue_s = [&](uint32_t n) {
+        const uint32_t st = n % NS, buf = js & 1u;
+        if (!(ok = tc_wait(&B.k_full[st], (n / NS) & 1u, abort_flag))) return;
+        if (js >= S::kSBufs && !(ok = tc_wait(&B.s_free[g][(js - S::kSBufs) & 1], ((js - S::kSBufs) >> 1) & 1u, abort_flag))) return;
+        tc_fence_after();
+        const uint64_t db = dk + st * NB * (S::kBlock / 16);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma_f16(ts + (js % S::kSBufs) * BK, dq + (k >> 2) * 1024 + 2 * (k & 3), db + (k >> 2) * (S::kBlock / 16) + 2 * (k & 3), id_s,
+                     k != 0 ? 1u : 0u);
+        tc_commit(&B.s_full[g][buf]);
+        tc_commit(&B.k_empty[st]);
+        ++js;
+      };
+      for (; ok && w.next(a); ++segment) {
+        const uint32_t ntiles = (w.key1 - w.key0 + BK - 1) / BK, n0 = number;
+        number += ntiles;
+        if (!(ok = tc_wait(&B.q_full, segment & 1u, abort_flag))) break;
+        if (SPLITQ && w.live_rows <= 128 * g) {  // no rows: the tiles are only given back
+          for (uint32_t n = n0; ok && n < number; ++n) {
+            ok = tc_wait(&B.k_full[n % NS], (n / NS) & 1u, abort_flag) && tc_wait(&B.v_full[n % NS], (n / NS) & 1u, abort_flag);
+            mbar_arrive(&B.k_empty[n % NS]);
+            mbar_arrive(&B.v_empty[n % NS]);
+          }
+          continue;
+        }
+        const uint32_t first = n0 + (SPLITQ ? 0 : g);
+        if (first < number) issue_s(first);
+        for (uint32_t n = first; ok && n < number; n += STEP) {
+          // S of the next tile first: it is computed while this one's exponentials run
+          if (n + STEP < number) issue_s(n + STEP);
+          const uint32_t st = n % NS, buf = jo & 1u;
+          if (!ok || !(ok = tc_wait(&B.v_full[st], (n / NS) & 1u, abort_flag) && tc_wait(&B.p_full[g][buf], (jo >> 1) & 1u, abort_flag))) break;
+          tc_fence_after();
+          const uint64_t da = dp + (jo % S::kPBufs) * (S::kPBytes / 16), db = dv + st * NB * (S::kBlock / 16);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) tc_mma_f16(to, da + (k >> 2) * 1024 + 2 * (k & 3), db + k * 128, id_o, n != first || k != 0 ? 1u : 0u);
+          tc_commit(&B.pv_done[g][buf]);
+          tc_commit(&B.v_empty[st]);
+          ++jo;
+        }
+      }
+      if (!ok) {
+        fail();
+        tc_commit(&B.drain[g]);
+        mbar_wait(&B.drain[g], 0, nullptr);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ loads
+    const int group = (warp - 10) / kLoadWarps;
+    const int tid = threadIdx.x - 32 * 10 - group * kLoadThreads;
+    constexpr int PER = BK * CPR / kLoadThreads;  // 16-byte pieces of a thread, of K and of V: each KPX keys on
+    constexpr int KPX = kLoadThreads / CPR;
+    static_assert(KPX % 8 == 0, "a thread's pieces have one swizzle");
+    // (rolled where the pieces need no registers of their own: the roles' code shares the instruction cache)
+    constexpr int ROLL = S::kInRegs ? PER : 1;
+    const int page_mask = (1 << a.pools.page_shift) - 1;
+    const int my_key = tid / CPR, my_c = tid % CPR;
+    uint32_t issued = 0, done = 0;  // of this group's tiles: the numbers group, group + 2, ...
+    uint32_t nodes = 0;             // bit i: the tile issued i tiles ago holds new tokens
+    float scale_of_tile = 0.f;
+    uint4 held[S::kInRegs ? 2 * PER : 1];  // (kInRegs: the tile under way)
+    bool ok = true;
+    // The page of a key of the segment, or -1 behind its last one; reports a page that is not there.
+    auto page_of = [&](int key) {
+      if (key >= w.key1) return -1;
+      const int p = __ldg(a.batch.page_table + w.b * a.batch.table_stride + (key >> a.pools.page_shift));
+      if (p >= 0 && p < a.pools.num_pages) return p;
+      atomicOr(a.err, kErrBadIndex);
+      return -1;
+    };
+    // asks for tile n of the segment, the one at `base`
+    auto issue = [&](uint32_t n, int base) {
+      const uint32_t at = CODES ? smem_u32(smem + S::kRawAt) + (n % (CODES && !S::kInRegs ? S::kRaw : 1)) * 2 * BK * RB + tid * 16
+                                : smem_u32(smem + S::kK) + ((n % NS) * NB + (my_c >> 3)) * S::kBlock + my_key * 128 + (((my_c & 7) ^ (my_key & 7)) << 4);
+      constexpr uint32_t TO_X = CODES ? kLoadThreads * 16 : KPX * 128, TO_V = CODES ? BK * RB : S::kV - S::kK;
+      auto fetch = [&](int x, long long byte, bool live) {
+        const uint8_t* k = static_cast<const uint8_t*>(a.pools.k) + byte;
+        const uint8_t* v = static_cast<const uint8_t*>(a.pools.v) + byte;
+        if constexpr (S::kInRegs) {
+          held[2 * x] = live ? __ldg(reinterpret_cast<const uint4*>(k)) : make_uint4(0u, 0u, 0u, 0u);
+          held[2 * x + 1] = live ? __ldg(reinterpret_cast<const uint4*>(v)) : make_uint4(0u, 0u, 0u, 0u);
+        } else {
+          cp16(at + x * TO_X, k, live);
+          cp16(at + TO_V + x * TO_X, v, live);
+        }
+      };
+      if ((1 << a.pools.page_shift) >= BK) {  // the tile is one run of its page
+        const int page = page_of(base);
+        const long long first = page >= 0 ? kv_slot(a.pools, page, w.kvh, base & page_mask) : 0;
+        const int live = page >= 0 ? w.key1 - base : 0;
+#pragma unroll ROLL
+        for (int x = 0; x < PER; ++x) {
+          const bool here = my_key + x * KPX < live;
+          fetch(x, here ? first * RB + tid * 16 + x * (kLoadThreads * 16) : 0, here);
+        }
+      } else {
+#pragma unroll ROLL
+        for (int x = 0; x < PER; ++x) {
+          const int page = page_of(base + my_key + x * KPX);
+          const long long slot = page >= 0 ? kv_slot(a.pools, page, w.kvh, (base + my_key + x * KPX) & page_mask) : 0;
+          fetch(x, page >= 0 ? slot * RB + my_c * 16 : 0, page >= 0);
+        }
+      }
+      if constexpr (CODES) {  // and scales: of key tid % BK, K's and V's by turns of BK threads
+#pragma unroll
+        for (int x = 0; x < 2 * BK / kLoadThreads; ++x) {
+          const int i = x * kLoadThreads + tid, key = base + (i & (BK - 1)), page = page_of(key);
+          const float* from = (i < BK ? a.pools.k_scale : a.pools.v_scale) + (page >= 0 ? kv_slot(a.pools, page, w.kvh, key & page_mask) : 0);
+          if constexpr (S::kRawScales)
+            cp4(smem_u32(smem + S::kRawScale) + ((n % S::kRaw) * 2 * BK + i) * 4, from, page >= 0);
+          else
+            scale_of_tile = page >= 0 ? *from : 0.f;
+        }
+      }
+      cp_commit();
+      nodes = nodes << 1 | (base + BK > w.ctx ? 1u : 0u);
+      ++issued;
+    };
+    // waits for the oldest tile under way and hands it to the products
+    auto finish = [&] {
+      const uint32_t n = LG * done + group;
+      const int st = n % NS;
+      if (issued - done == S::kAhead)
+        cp_wait<S::kAhead - 1>();
+      else
+        cp_wait<0>();
+      if constexpr (CODES) {
+#pragma unroll
+        for (int x = 0; x < 2 * BK / kLoadThreads; ++x) {
+          const int i = x * kLoadThreads + tid;
+          reinterpret_cast<float*>(smem + S::kScale)[(n % S::kScaleSlots) * 2 * BK + i] =
+              S::kRawScales ? reinterpret_cast<const float*>(smem + S::kRawScale)[(n % (S::kRaw + !S::kRaw)) * 2 * BK + i] : scale_of_tile;
+        }
+        const uint32_t from = smem_u32(smem + S::kRawAt) + (n % (S::kRaw + !S::kRaw)) * 2 * BK * RB + tid * 16;
+        const uint32_t to = smem_u32(smem + S::kK) + (st * NB + (my_c >> 2)) * S::kBlock + my_key * 128;
+        const uint32_t to0 = (((2 * my_c) & 7) ^ (my_key & 7)) << 4, to1 = (((2 * my_c + 1) & 7) ^ (my_key & 7)) << 4;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (n >= NS && !warp_wait(kv ? &B.v_empty[st] : &B.k_empty[st], ((n / NS) - 1) & 1u)) return false;
+#pragma unroll
+          for (int x = 0; x < PER; ++x) {
+            uint4 v;
+            if constexpr (S::kInRegs)
+              v = held[2 * x + kv];
+            else
+              v = lds128(from + kv * BK * RB + x * kLoadThreads * 16);
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[2 * i] = code_pair_bf16<FMT>(e[i], 0);
+              o[2 * i + 1] = code_pair_bf16<FMT>(e[i], 1);
+            }
+            const uint32_t dst = to + (kv ? S::kV - S::kK : 0) + x * KPX * 128;
+            sts128(dst + to0, make_uint4(o[0], o[1], o[2], o[3]));
+            sts128(dst + to1, make_uint4(o[4], o[5], o[6], o[7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv ? &B.v_full[st] : &B.k_full[st]);
+        }
+      } else {
+        if ((nodes >> (issued - done - 1)) & 1u) {
+          const uint32_t at = smem_u32(smem + S::kV) + (st * NB + (my_c >> 3)) * S::kBlock + my_key * 128 + (((my_c & 7) ^ (my_key & 7)) << 4);
+#pragma unroll 1
+          for (int x = 0; x < PER; ++x) {
+            const uint4 v = lds128(at + x * KPX * 128);
+            uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((e[i] & 0x7F80u) == 0x7F80u) e[i] &= 0xFFFF0000u, odd = true;
+              if ((e[i] & 0x7F800000u) == 0x7F800000u) e[i] &= 0x0000FFFFu, odd = true;
+            }
+            if (odd) {
+              sts128(at + x * KPX * 128, make_uint4(e[0], e[1], e[2], e[3]));
+              atomicExch(&B.odd_values, 1);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&B.k_full[st]);
+          mbar_arrive(&B.v_full[st]);
+        }
+      }
+      ++done;
+      return true;
+    };
+    while (ok && w.next(a)) {
+      const int ntiles = (w.key1 - w.key0 + BK - 1) / BK;
+      const uint32_t first = number;
+      number += ntiles;
+      for (int t = (group - first) & (LG - 1); ok && t < ntiles; t += LG) {
+        const uint32_t n = first + t;
+        if (issued - done == S::kAhead) ok = finish();
+        if constexpr (!CODES) {
+          // The stage's last tile must be done with. Where it is not yet, the tiles under way
+          // are handed over first: the products may be waiting for just those.
+          if (ok && n >= NS) {
+            const uint32_t parity = ((n / NS) - 1) & 1u;
+            auto free_now = [&] {
+              int f = 1;
+              if (lane == 0) f = mbar_test_wait(&B.k_empty[n % NS], parity) && mbar_test_wait(&B.v_empty[n % NS], parity);
+              return __shfl_sync(0xffffffffu, f, 0) != 0;
+            };
+            while (ok && done < issued && !free_now()) ok = finish();
+            ok = ok && warp_wait(&B.k_empty[n % NS], parity) && warp_wait(&B.v_empty[n % NS], parity);
+          }
+        }
+        if (ok) issue(n, w.key0 + t * BK);
+      }
+    }
+    while (ok && done < issued) ok = finish();
+    cp_wait<0>();
+    if (!ok) fail();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, S::kTmemCols);
+}
+
+template <int HD, int FMT, bool SPLITQ>
+TreeTcVariant tc_variant() {
+  using S = TcShape<HD, FMT, SPLITQ>;
+  return TreeTcVariant{tree_attention_tc_kernel<HD, FMT, SPLITQ>, S::kRows, S::kThreads, S::kSmem};
+}
+
+template <int FMT>
+TreeTcVariant tc_variant_of(int head_dim, int64_t rows) {
+  if (head_dim == 128) return tc_variant<128, FMT, false>();
+  return rows <= 128 ? tc_variant<64, FMT, false>() : tc_variant<64, FMT, true>();
+}
+
+}  // namespace
+
+TreeTcVariant tree_tc_variant(int format, int head_dim, int64_t rows) {
+  return format == NCM_KV_BF16   ? tc_variant_of<NCM_KV_BF16>(head_dim, rows)
+         : format == NCM_KV_INT8 ? tc_variant_of<NCM_KV_INT8>(head_dim, rows)
+                                 : tc_variant_of<NCM_KV_E4M3>(head_dim, rows);
+}
+
+}  // namespace ncm

@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import context, need_rows, need_vec, raw_stream
+from .device import context_of, empty_rows, need_rows, need_vec, raw_stream
 
 bf16, i32 = torch.bfloat16, torch.int32
 FORMATS = {bf16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
@@ -59,6 +59,7 @@ class KVCache:
         c.format = FORMATS[k.dtype]
         c.num_pages, c.kv_heads, c.page_size, c.head_dim = k.shape
         self._ref = ctypes.byref(c)
+        self._workspaces = {}  # sizes by call shape
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = bf16,
@@ -98,7 +99,7 @@ def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, token_start: torch.
     if v.shape[0] != k.shape[0]:
         raise ValueError(f"k and v must have the same rows, got {k.shape[0]} and {v.shape[0]}")
     b = _batch(cache, token_start, kv_lens, page_table, k.shape[0])
-    _lib.call("ncm_kv_cache_append", context(dev), cache._ref, ctypes.byref(b), k.data_ptr(), ks, v.data_ptr(), vs,
+    _lib.call("ncm_kv_cache_append", context_of(dev), cache._ref, ctypes.byref(b), k.data_ptr(), ks, v.data_ptr(), vs,
               raw_stream(dev))
 
 
@@ -113,13 +114,13 @@ def gather(cache: KVCache, row_start: torch.Tensor, page_table: torch.Tensor, ro
     if out_k is None or out_v is None:
         if rows is None:
             raise ValueError("rows is needed without out_k and out_v")
-        out_k = torch.empty((rows, cache.width), dtype=bf16, device=dev) if out_k is None else out_k
-        out_v = torch.empty((rows, cache.width), dtype=bf16, device=dev) if out_v is None else out_v
+        out_k = empty_rows(rows, cache.width, bf16, dev) if out_k is None else out_k
+        out_v = empty_rows(rows, cache.width, bf16, dev) if out_v is None else out_v
     ks, vs = need_rows(out_k, bf16, "out_k", dev, cache.width), need_rows(out_v, bf16, "out_v", dev, cache.width)
     if out_v.shape[0] != out_k.shape[0] or (rows is not None and out_k.shape[0] != rows):
         raise ValueError("out_k and out_v must have the same rows")
     b = _batch(cache, row_start, None, page_table, out_k.shape[0])
-    _lib.call("ncm_kv_cache_gather", context(dev), cache._ref, ctypes.byref(b),
+    _lib.call("ncm_kv_cache_gather", context_of(dev), cache._ref, ctypes.byref(b),
               need_vec(begin, i32, "begin", dev, b.batch), out_k.data_ptr(), ks, out_v.data_ptr(), vs, raw_stream(dev))
     return out_k, out_v
 
@@ -150,17 +151,25 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
             raise ValueError(f"tree_mask must be a contiguous int32 [{T}, words] tensor on {dev}")
         words = tree_mask.shape[1]
     if out is None:
-        out = torch.empty((T, width), dtype=bf16, device=dev)
-    os_ = need_rows(out, bf16, "out", dev, width)
-    if out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
-    lse = torch.empty((T, heads), dtype=torch.float32, device=dev) if return_lse else None
-    ctx, bref = context(dev), ctypes.byref(b)
-    size = ctypes.c_uint64()
-    _lib.call("ncm_tree_attention_workspace", ctx, cache._ref, bref, heads, max_nodes, ctypes.byref(size))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
+        out, os_ = empty_rows(T, width, bf16, dev), width
+    else:
+        os_ = need_rows(out, bf16, "out", dev, width)
+        if out.shape[0] != T:
+            raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
+    lse = empty_rows(T, heads, torch.float32, dev) if return_lse else None
+    ctx, bref = context_of(dev), ctypes.byref(b)
+    # the size depends on nothing but these numbers
+    size = cache._workspaces.get((heads, max_nodes, b.table_width, b.batch))
+    if size is None:
+        n = ctypes.c_uint64()
+        _lib.call("ncm_tree_attention_workspace", ctx, cache._ref, bref, heads, max_nodes, ctypes.byref(n))
+        if len(cache._workspaces) >= 256:
+            cache._workspaces.clear()
+        size = cache._workspaces[heads, max_nodes, b.table_width, b.batch] = n.value
+    # (new memory for every call: calls on other streams and captured graphs share none)
+    ws = empty_rows(1, size, torch.uint8, dev) if size else None
     _lib.call("ncm_tree_attention", ctx, cache._ref, bref, q.data_ptr(), qs,
               None if tree_mask is None else tree_mask.data_ptr(), words, heads, max_nodes,
               hd ** -0.5 if scale is None else scale, out.data_ptr(), os_, None if lse is None else lse.data_ptr(),
-              None if ws is None else ws.data_ptr(), size.value, raw_stream(dev))
+              None if ws is None else ws.data_ptr(), size, raw_stream(dev))
     return (out, lse) if return_lse else out

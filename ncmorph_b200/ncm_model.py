@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .device import context, need, need_rows, need_vec, ptr, raw_stream, stream_of
+from .device import context, context_of, empty_rows, need, need_rows, need_vec, ptr, raw_stream, stream_of
 
 MASK_MODES = {"causal": 0, "block_diagonal": 1, "block_causal": 2}
 bf16 = torch.bfloat16
@@ -89,11 +89,12 @@ def rope_bf16(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: 
         raise ValueError(f"cos and sin must be contiguous and of one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
     pos = need_vec(positions, torch.int32, "positions", dev, T)
     if out is None:
-        out = torch.empty((T, width), dtype=bf16, device=dev)
-    out_stride = need_rows(out, bf16, "out", dev, width)
-    if out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
-    _lib.call("ncm_rope_bf16", context(dev), x.data_ptr(), stride, out.data_ptr(), out_stride, pos, cos.data_ptr(),
+        out, out_stride = empty_rows(T, width, bf16, dev), width
+    else:
+        out_stride = need_rows(out, bf16, "out", dev, width)
+        if out.shape[0] != T:
+            raise ValueError(f"out must have {T} rows, got {out.shape[0]}")
+    _lib.call("ncm_rope_bf16", context_of(dev), x.data_ptr(), stride, out.data_ptr(), out_stride, pos, cos.data_ptr(),
               sin.data_ptr(), P, T, heads, head_dim, rotary, interleaved, inverse, raw_stream(dev))
     return out
 
@@ -310,12 +311,13 @@ def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, tok
     R, V = logits.shape
     stride = need_rows(logits, logits.dtype, "logits", dev, V)
     if out is None:
-        out = torch.empty((R, V), dtype=torch.float32, device=dev)
-    if not isinstance(out, torch.Tensor) or out.dtype not in (torch.float32, logits.dtype):
-        raise TypeError(f"out must be a float32 or {logits.dtype} tensor")
-    out_stride = need_rows(out, out.dtype, "out", dev, V)
-    if tuple(out.shape) != (R, V):
-        raise ValueError(f"out must have shape {(R, V)}, got {tuple(out.shape)}")
+        out, out_stride = empty_rows(R, V, torch.float32, dev), V
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype not in (torch.float32, logits.dtype):
+            raise TypeError(f"out must be a float32 or {logits.dtype} tensor")
+        out_stride = need_rows(out, out.dtype, "out", dev, V)
+        if tuple(out.shape) != (R, V):
+            raise ValueError(f"out must have shape {(R, V)}, got {tuple(out.shape)}")
     i32, f32 = torch.int32, torch.float32
     r = _lib.LogitRules()
     if tokens is not None:
@@ -342,6 +344,6 @@ def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, tok
         r.allowed_rows = need_vec(allowed_rows, i32, "allowed_rows", dev, R)
     elif allowed_rows is not None:
         raise ValueError("allowed_rows needs allowed")
-    _lib.call("ncm_logits_process", context(dev), logits.data_ptr(), LOGIT_TYPES[logits.dtype], stride, out.data_ptr(),
+    _lib.call("ncm_logits_process", context_of(dev), logits.data_ptr(), LOGIT_TYPES[logits.dtype], stride, out.data_ptr(),
               LOGIT_TYPES[out.dtype], out_stride, R, V, ctypes.byref(r), raw_stream(dev))
     return out

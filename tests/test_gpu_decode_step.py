@@ -247,6 +247,29 @@ def test_append_of_hard_rows(cuda_dev, dtype):
         assert torch.equal(got.cpu()[ok], want[ok])
 
 
+@pytest.mark.parametrize("dtype", FORMATS[1:])
+def test_codes_of_every_ratio(cuda_dev, dtype):
+    """Every pair of bf16 mantissas, near and far exponents: the codes and scales of exact arithmetic."""
+    A = torch.arange(128, 256).float()
+    rows = []
+    for shift in (0, 1, 2, 5, 7, 9):
+        other = torch.arange(128, 256).float() * 2.0 ** -shift
+        for i in range(128):
+            x = torch.minimum(other, A[i]).view(2, 64).clone()
+            x[:, 63] = A[i]
+            rows.append(x * torch.tensor([[1.0], [-1.0]]))
+    x = torch.cat(rows)
+    x = (x * 2.0 ** torch.randint(-60, 60, (x.shape[0], 1)).float()).to(torch.bfloat16)
+    w = World(cuda_dev, dtype, [x.shape[0]], [x.shape[0]], 1, 64, 128)
+    w.k = w.v = x
+    w.fill()
+    codes, scale = quantise_ref(x.view(-1, 1, 64), dtype)
+    table = w.table_cpu[0, : -(-x.shape[0] // 128)].long()
+    got = w.cache.k.cpu()[table].reshape(-1, 64)[: x.shape[0]].double()
+    assert torch.equal(got, codes[:, 0])
+    assert torch.equal(w.cache.k_scale.cpu()[table].reshape(-1)[: x.shape[0]], scale[:, 0])
+
+
 def test_gather_ranges_and_qkv_columns(cuda_dev):
     """A window of each sequence, into the K and V columns of fused QKV rows;
     rows behind the last sequence stay as they were."""
@@ -447,33 +470,40 @@ def test_hidden_and_empty(cuda_dev, dtype, rows):
     assert torch.all(out[n - 1] == 0) and torch.all(lse[n - 1] == -math.inf)
 
 
-def test_seen_infinite_values(cuda_dev):
+@pytest.mark.parametrize("n,L,hd", [(6, 70, 64), (70, 150, 64), (140, 500, 64), (90, 800, 128)])
+def test_seen_infinite_values(cuda_dev, n, L, hd):
     """A finite key whose value row holds an infinity reaches the rows that see it, and no others."""
     from ncmorph_b200 import kv_cache
-    w = World(cuda_dev, torch.bfloat16, [70], [6], 1, 64, 16)
-    w.v[66, 5], w.v[67, 9], w.v[30, 40] = math.inf, -math.inf, math.inf
+    w = World(cuda_dev, torch.bfloat16, [L], [n], 1, hd, 16)
+    c = L - n
+    w.v[c + 2, 5], w.v[c + 3, 9], w.v[30, 40], w.v[c - 1, 50] = math.inf, -math.inf, math.inf, -math.inf
     w.fill()
-    q = torch.randn((6, 64), generator=w.g).to(torch.bfloat16)
-    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=6, return_lse=True)
+    q = torch.randn((n, hd), generator=w.g).to(torch.bfloat16)
+    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=n, return_lse=True)
     out = out.cpu()
-    inf = torch.isinf(out)
-    want = torch.zeros((6, 64), dtype=torch.bool)
-    want[2:, 5] = want[3:, 9] = want[:, 40] = True
-    assert torch.equal(inf, want) and not torch.isnan(out).any()
+    want = torch.zeros((n, hd), dtype=torch.bool)
+    want[2:, 5] = want[3:, 9] = want[:, 40] = want[:, 50] = True
+    assert torch.equal(torch.isinf(out), want) and not torch.isnan(out).any()
+    w.v[~torch.isfinite(w.v)] = 0.0
+    o, l, to, tl = attend_ref(w, q, 1, None, hd ** -0.5)
+    assert torch.all(((out.double() - o).abs() <= to) | want) and torch.all((lse.cpu().double() - l).abs() <= tl)
 
 
 @pytest.mark.parametrize("dtype", FORMATS)
-def test_sharp_and_wide_scores(cuda_dev, dtype):
+@pytest.mark.parametrize("new,hd", [((2, 1), 128), ((30, 1), 128), ((30, 17), 64), ((64, 40), 64)])
+def test_sharp_and_wide_scores(cuda_dev, dtype, new, hd):
     """Scores far apart: the maximum moves often, and late."""
     from ncmorph_b200 import kv_cache
-    w = World(cuda_dev, dtype, [1300, 400], [2, 1], 1, 128, 32, seed=5)
+    w = World(cuda_dev, dtype, [1300, 400], list(new), 1, hd, 32, seed=5)
     ramp = torch.cat([torch.linspace(0.1, 4, n) for n in (1300, 400)])[:, None]
     w.k = (w.k.float() * ramp).to(torch.bfloat16)
     w.v = (w.v.float() * torch.exp(4 * torch.randn((1700, 1), generator=w.g))).to(torch.bfloat16)
     w.fill()
-    q = (3 * torch.randn((3, 4 * 128), generator=w.g)).to(torch.bfloat16)
-    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=2, return_lse=True)
-    check_attention(out, lse, attend_ref(w, q, 4, None, 128 ** -0.5))
+    for scale in (hd ** -0.5, -0.07, 0.0):
+        q = (3 * torch.randn((w.T, 4 * hd), generator=w.g)).to(torch.bfloat16)
+        out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=max(new), scale=scale,
+                                           return_lse=True)
+        check_attention(out, lse, attend_ref(w, q, 4, None, scale))
 
 
 def test_many_sequences_and_strided_rows(cuda_dev):
