@@ -21,7 +21,7 @@ namespace ncm {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowTokens = 32;  // rows that a block moves at most
+constexpr int kRowTokens = 16;  // rows of a chunk at most
 
 __device__ __forceinline__ uint16_t pack_e4m3x2(float lo, float hi) {
   uint16_t r;
@@ -78,18 +78,22 @@ __device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top, float* 
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= pre;
   }
+  const unsigned long long f2 = f2_pack(factor, factor), s2 = f2_pack(65.f, 65.f), n2 = f2_pack(-1.f, -1.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __fmul_rn(y[i], factor), c = __fmul_rn(q, 65.f);
-    y[i] = __fsub_rn(c, __fsub_rn(c, q));  // q rounded to 18 bits
+  for (int i = 0; i < 8; i += 2) {  // q = y factor rounded to 18 bits: c - (c - q) with c = 65 q
+    const unsigned long long q = f2_mul(f2_pack(y[i], y[i + 1]), f2), c = f2_mul(q, s2);
+    unsigned long long r = f2_fma(f2_fma(q, n2, c), n2, c);
+    // 1.5 * 2^23 + q rounds q to a whole number, ties to even; its low byte is the code
+    if constexpr (FMT == NCM_KV_INT8) r = f2_add(r, f2_pack(12582912.f, 12582912.f));
+    f2_unpack(r, y[i], y[i + 1]);
   }
   uint32_t out[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if constexpr (FMT == NCM_KV_INT8) {
-      uint32_t b[4];  // 1.5 * 2^23 + y rounds y to a whole number, ties to even; its low byte is the code
+      uint32_t b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(y[4 * h + i], 12582912.f));
+      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(y[4 * h + i]);
       out[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     } else {
       out[h] = pack_e4m3x2(y[4 * h], y[4 * h + 1]) | (static_cast<uint32_t>(pack_e4m3x2(y[4 * h + 2], y[4 * h + 3])) << 16);
@@ -100,25 +104,26 @@ __device__ __forceinline__ uint2 quantise8(const uint4& v, uint32_t top, float* 
 
 template <int FMT>
 __device__ __forceinline__ uint4 dequantise8(uint32_t lo, uint32_t hi, float scale) {
-  float y[8];
   const uint32_t w[2] = {lo, hi};
+  const unsigned long long s2 = f2_pack(scale, scale);
+  uint32_t out[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if constexpr (FMT == NCM_KV_INT8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)  // 2^23 + 128 + code, less 2^23 + 128
-        y[4 * h + i] = __uint_as_float(__byte_perm(w[h] ^ 0x80808080u, 0x4B000000u, 0x7440 | i)) - 8388736.f;
+  for (int h = 0; h < 4; ++h) {
+    unsigned long long y;
+    if constexpr (FMT == NCM_KV_INT8) {  // 2^23 + 128 + code, less 2^23 + 128
+      const uint32_t x = w[h >> 1] ^ 0x80808080u;
+      y = f2_add(f2_pack(__uint_as_float(__byte_perm(x, 0x4B000000u, 0x7440 | (2 * (h & 1)))),
+                         __uint_as_float(__byte_perm(x, 0x4B000000u, 0x7440 | (2 * (h & 1) + 1)))),
+                 f2_pack(-8388736.f, -8388736.f));
     } else {
-      const float2 a = f16x2_to_f32(e4m3x2_to_f16x2(static_cast<uint16_t>(w[h])));
-      const float2 b = f16x2_to_f32(e4m3x2_to_f16x2(static_cast<uint16_t>(w[h] >> 16)));
-      y[4 * h] = a.x;
-      y[4 * h + 1] = a.y;
-      y[4 * h + 2] = b.x;
-      y[4 * h + 3] = b.y;
+      const float2 a = f16x2_to_f32(e4m3x2_to_f16x2(static_cast<uint16_t>(w[h >> 1] >> (16 * (h & 1)))));
+      y = f2_pack(a.x, a.y);
     }
+    float p, q;
+    f2_unpack(f2_mul(y, s2), p, q);
+    out[h] = pack_rn_bf16x2(p, q);
   }
-  return make_uint4(pack_rn_bf16x2(y[0] * scale, y[1] * scale), pack_rn_bf16x2(y[2] * scale, y[3] * scale),
-                    pack_rn_bf16x2(y[4] * scale, y[5] * scale), pack_rn_bf16x2(y[6] * scale, y[7] * scale));
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 struct RowsArgs {
@@ -164,20 +169,17 @@ __device__ __forceinline__ int slot_of_row(const RowsArgs& a, long long t) {
   return (page << a.pools.page_shift) + (pos & ((1 << a.pools.page_shift) - 1));
 }
 
-// A block resolves its rows' slots (one lane each) and then moves them. A
-// thread keeps its eight values of a row (a head of the keys or the values:
-// blockIdx.y picks the part of the row) and walks over the block's rows, BATCH of
-// them loaded before the first is stored.
+// A block moves chunks of `tokens` rows: one lane each resolves the next chunk's
+// slots while this one's rows are on their way. A thread keeps its eight values
+// of a row (a head of the keys or the values: blockIdx.y picks the part of the
+// row) and walks over the chunk's rows, BATCH of them loaded before the first is stored.
 template <int FMT, int HD, bool APPEND>
 __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) {
-  __shared__ int slots[kRowTokens];
+  __shared__ int slot_of[2][kRowTokens];
   pdl_wait();
   pdl_launch_dependents();
   constexpr bool CODES = FMT != NCM_KV_BF16;
-  constexpr int LPR = HD / 8, EB = CODES ? 1 : 2, BATCH = APPEND ? 4 : 8;
-  const long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
-  for (int i = threadIdx.x; i < a.tokens; i += kRowThreads) slots[i] = slot_of_row<APPEND>(a, t0 + i);
-  __syncthreads();
+  constexpr int LPR = HD / 8, EB = CODES ? 1 : 2, BATCH = APPEND ? 4 : 2;
   const int lane_row = threadIdx.x / LPR, piece = threadIdx.x % LPR;
   const int e = blockIdx.y * a.part_rows + lane_row % a.part_rows;  // head row: keys, then values
   const int first = lane_row / a.part_rows, step = (kRowThreads / LPR) / a.part_rows;  // this thread's tokens
@@ -185,9 +187,16 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
   const bool is_v = e >= a.pools.kv_heads;
   const int h = is_v ? e - a.pools.kv_heads : e;
   const long long stride = is_v ? a.v_stride : a.k_stride;
-  uint16_t* rows = (is_v ? a.v : a.k) + t0 * stride + h * HD + piece * 8;
   uint8_t* codes = static_cast<uint8_t*>(is_v ? a.pools.v : a.pools.k) + piece * 8 * EB;
   float* scales = is_v ? a.pools.v_scale : a.pools.k_scale;
+  long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
+  const long long t_step = static_cast<long long>(gridDim.x) * a.tokens;
+  if (threadIdx.x < a.tokens) slot_of[0][threadIdx.x] = slot_of_row<APPEND>(a, t0 + threadIdx.x);
+  __syncthreads();
+  for (int turn = 0; t0 < a.batch.rows; t0 += t_step, turn ^= 1) {
+  const int* slots = slot_of[turn];
+  uint16_t* rows = (is_v ? a.v : a.k) + t0 * stride + h * HD + piece * 8;
+  if (threadIdx.x < a.tokens) slot_of[turn ^ 1][threadIdx.x] = slot_of_row<APPEND>(a, t0 + t_step + threadIdx.x);
   for (int i0 = 0; i0 < a.tokens; i0 += BATCH * step) {
     uint4 x[BATCH];
     float scale[BATCH];
@@ -230,6 +239,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
       }
     }
   }
+  __syncthreads();
+  }
 }
 
 template <bool APPEND>
@@ -239,6 +250,7 @@ int launch_rows(ncm_ctx* ctx, const ncm_kv_cache_t* c, RowsArgs& a, cudaStream_t
   a.tokens = static_cast<int>(std::min<int64_t>(kRowTokens, std::max<int64_t>(1, a.batch.rows / (4 * ctx->num_sms))));
   a.part_rows = std::min(2 * c->kv_heads, kRowThreads / (c->head_dim / 8));
   const int parts = ceil_div(2 * c->kv_heads, a.part_rows);
+  const int blocks = std::min(ceil_div(a.batch.rows, a.tokens), std::max(1, 8 * ctx->num_sms / parts));
   a.err = ctx->d_err;
   using Kernel = void (*)(const RowsArgs);
   static const Kernel table[3][2] = {
@@ -246,8 +258,7 @@ int launch_rows(ncm_ctx* ctx, const ncm_kv_cache_t* c, RowsArgs& a, cudaStream_t
       {kv_rows_kernel<NCM_KV_INT8, 64, APPEND>, kv_rows_kernel<NCM_KV_INT8, 128, APPEND>},
       {kv_rows_kernel<NCM_KV_E4M3, 64, APPEND>, kv_rows_kernel<NCM_KV_E4M3, 128, APPEND>}};
   Launch _launch(ctx, KID_KV_CACHE, st);
-  NCM_CUDA_TRY(launch_pdl(table[c->format][c->head_dim == 128], dim3(ceil_div(a.batch.rows, a.tokens), parts), dim3(kRowThreads), 0,
-                          st, 1, a));
+  NCM_CUDA_TRY(launch_pdl(table[c->format][c->head_dim == 128], dim3(blocks, parts), dim3(kRowThreads), 0, st, 1, a));
   return NCM_OK;
 }
 

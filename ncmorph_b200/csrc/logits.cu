@@ -6,7 +6,11 @@
 // slice's tokens of the row's history in shared memory (bit 31: seen in the
 // prompt; the rest: times produced; integer atomics, so the order does not
 // matter) and finds the first of its bias entries for each token. Then it
-// changes and writes. Everything is f32, in separate operations in the documented order.
+// changes and writes. Tokens with a bias are written again, by the thread that
+// holds their first entry, so that no thread waits for one token's bias after
+// another's. What a block waits for is asked for together: the row's numbers, then
+// the first eight tokens of the history and the first bias entry of every thread.
+// Everything is f32, in separate operations in the documented order.
 //
 // Bound: memory, each logit read and written once. The history is read once
 // per slice (from L2 after the first).
@@ -42,6 +46,9 @@ __device__ __forceinline__ void row_range(const int32_t* start, long long total,
     *lo = *hi = 0;
   }
 }
+
+__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = static_cast<uint16_t>(pack_rn_bf16x2(v, 0.f)); }
 
 // Eight neighbouring logits from / to a row; `left` of them exist. VEC: the row is 16-byte aligned.
 template <bool VEC>
@@ -112,7 +119,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs 
   const ncm_logit_rules_t& R = a.r;
   const bool history = R.tokens != nullptr, biased = R.bias != nullptr;
   uint32_t* count = sh;
-  uint32_t* entry = sh + (history ? slice : 0);
+  uint32_t* entry = sh + slice;  // (with biases; the counts' place then exists without a history, too)
   int t_lo = 0, t_hi = 0, b_lo = 0, b_hi = 0;
   if (history) {
     row_range(R.token_start, R.num_tokens, r, &t_lo, &t_hi, a.err);
@@ -144,13 +151,23 @@ __global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs 
       atomicOr(a.err, kErrBadIndex);
     }
   }
+  // (the first tokens and the first bias entry of this thread, ahead of their use)
+  constexpr int AHEAD = 8;
+  int ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = t_lo + k * threads + threadIdx.x;
+    ahead[k] = i < t_hi ? __ldg(R.tokens + i) : 0;
+  }
+  const int my = b_lo + threadIdx.x;
+  const unsigned my_id = my < b_hi ? static_cast<unsigned>(__ldg(R.bias_ids + my)) : 0u;
+  const float my_bias = my < b_hi ? __ldg(R.bias + my) : 0.f;
   __syncthreads();
   const unsigned first = static_cast<unsigned>(v0), un = static_cast<unsigned>(n);
   const int t_mid = t_lo + min(max(prompt, 0), t_hi - t_lo);
   bool bad = false;
-#pragma unroll 4
-  for (int i = t_lo + threadIdx.x; i < t_hi; i += threads) {
-    const unsigned id = static_cast<unsigned>(__ldg(R.tokens + i)), j = id - first;
+  auto note = [&](int i, int token) {
+    const unsigned id = static_cast<unsigned>(token), j = id - first;
     if (j < un) {
       if (i < t_mid)
         atomicOr(count + j, kInPrompt);
@@ -158,18 +175,26 @@ __global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs 
         atomicAdd(count + j, 1u);
     }
     bad |= id >= static_cast<unsigned>(a.vocab);
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = t_lo + k * threads + threadIdx.x;
+    if (i < t_hi) note(i, ahead[k]);
   }
+#pragma unroll 4
+  for (int i = t_lo + AHEAD * threads + threadIdx.x; i < t_hi; i += threads) note(i, __ldg(R.tokens + i));
+  auto id_of = [&](int i) { return i == my ? my_id : static_cast<unsigned>(__ldg(R.bias_ids + i)); };
   // the first entry of each token, then whether there are more
-  for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
-    const unsigned id = static_cast<unsigned>(__ldg(R.bias_ids + i)), j = id - first;
+  for (int i = my; i < b_hi; i += threads) {
+    const unsigned id = id_of(i), j = id - first;
     if (j < un) atomicMax(entry + j, kFirstEntry - static_cast<unsigned>(i - b_lo));
     bad |= id >= static_cast<unsigned>(a.vocab);
   }
   if (bad && blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
   __syncthreads();
   if (b_hi > b_lo) {
-    for (int i = b_lo + threadIdx.x; i < b_hi; i += threads) {
-      const unsigned j = static_cast<unsigned>(__ldg(R.bias_ids + i)) - first;
+    for (int i = my; i < b_hi; i += threads) {
+      const unsigned j = id_of(i) - first;
       if (j < un && (entry[j] & ~kRepeated) != kFirstEntry - static_cast<unsigned>(i - b_lo)) atomicOr(entry + j, kRepeated);
     }
     __syncthreads();
@@ -194,26 +219,33 @@ __global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs 
         }
       }
     }
-    if (b_hi > b_lo) {
+    if (b_hi > b_lo) {  // tokens with a bias: their logits take their counts' place
       uint32_t c[8];
       *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(entry + i);
       *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(entry + i + 4);
       if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0u) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (c[e] == 0u) continue;
-          const int at = b_lo + static_cast<int>(kFirstEntry - (c[e] & ~kRepeated));
-          x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + at));
-          if (c[e] & kRepeated)
-            for (int k = at + 1; k < b_hi; ++k)
-              if (__ldg(R.bias_ids + k) == v0 + i + e) x[g][e] = __fadd_rn(x[g][e], __ldg(R.bias + k));
-        }
+        for (int e = 0; e < 8; ++e)
+          if (c[e] != 0u) count[i + e] = __float_as_uint(x[g][e]);
       }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (!((bits[g] >> e) & 1u)) x[g][e] = -__uint_as_float(0x7F800000u);
     store8<VEC>(out + i, n - i, x[g]);
+  }
+  if (b_hi > b_lo) {
+    __syncthreads();  // (orders the stores above before the ones below, too)
+    for (int i = my; i < b_hi; i += threads) {
+      const unsigned id = id_of(i), j = id - first;
+      if (j >= un || (entry[j] & ~kRepeated) != kFirstEntry - static_cast<unsigned>(i - b_lo)) continue;
+      float y = __fadd_rn(__uint_as_float(count[j]), i == my ? my_bias : __ldg(R.bias + i));
+      if (entry[j] & kRepeated)
+        for (int k = i + 1; k < b_hi; ++k)
+          if (static_cast<unsigned>(__ldg(R.bias_ids + k)) == id) y = __fadd_rn(y, __ldg(R.bias + k));
+      if (mask != nullptr && !((__ldg(mask + (j >> 5)) >> (j & 31)) & 1u)) y = -__uint_as_float(0x7F800000u);
+      store_logit(out + j, y);
+    }
   }
 }
 
@@ -267,7 +299,7 @@ extern "C" int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dt
     threads /= 2;
   }
   const int slice = threads * 8 * groups;
-  const size_t smem = sizeof(uint32_t) * slice * ((r.tokens != nullptr) + (r.bias != nullptr));
+  const size_t smem = sizeof(uint32_t) * slice * (r.bias != nullptr ? 2 : r.tokens != nullptr ? 1 : 0);
   const bool vec = aligned_to(logits, 16) && aligned_to(out, 16) && stride * isz % 16 == 0 && out_stride * osz % 16 == 0;
   using Kernel = void (*)(const LogitArgs);
   static const Kernel table[3][2][2] = {
