@@ -549,7 +549,8 @@ NCM_API int ncm_rvq_level_noalloc_status(ncm_stream_t stream, int32_t* flags);
  * packages/kernels/root.zig:615-633; ncm_attention_bf16 keeps that). `inverse`
  * rotates by the negative angle: the gradient of the forward rotation.
  * Columns rotary_dim .. head_dim are copied. y may be x with the same
- * stride (in place); other overlaps are refused. A position outside
+ * stride (in place); where else the two ranges of rows overlap, column slices of
+ * one buffer included, the call is refused. A position outside
  * [0, table_rows) makes ncm_sync report NCM_ERANGE and leaves its row
  * unwritten. rotary_dim even, <= head_dim <= 1024; any alignment of whole elements. */
 NCM_API int ncm_rope_bf16(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride, uint16_t* y, int64_t y_stride,
@@ -583,7 +584,7 @@ typedef struct ncm_kv_cache {
  * slot p % page_size of page page_table[b * table_stride + p / page_size];
  * table_width entries per sequence may be read. A sequence whose numbers do
  * not fit (a negative count, more new tokens than keys, rows or keys past
- * the end) is skipped, a page outside [0, num_pages) is not touched, and both make
+ * the end, more than 2^30 keys) is skipped, a page outside [0, num_pages) is not touched, and both make
  * ncm_sync report NCM_ERANGE. */
 typedef struct ncm_kv_batch {
   const int32_t* token_start; /* [batch + 1] */
@@ -603,7 +604,8 @@ typedef struct ncm_kv_batch {
  *   e4m3: code = e4m3(448 x / A),  scale = A / 448
  * nearest, ties to even, exactly as in real arithmetic; A = 0 stores zeros
  * with scale 1, and a row holding a NaN or an infinity stores zeros with scale
- * NaN (it reads back as NaN). Two positions that the page tables map to one
+ * NaN (it reads back as NaN). The e4m3 codes 0x7F and 0xFF are never stored, and
+ * what the functions below make of them is not specified. Two positions that the page tables map to one
  * slot leave one of the two there, and not always the same one. */
 NCM_API int ncm_kv_cache_append(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                 const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
@@ -627,10 +629,14 @@ NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, con
  * per query head (head h reads kv head h / (heads / kv_heads), as
  * ncm_attention_bf16 does); a node that sees nothing gets zeros and -inf. q and
  * out [rows, heads * head_dim] bf16 (row strides in elements, multiples of 8;
- * 16-byte aligned), lse [rows, heads] f32 or NULL. max_nodes bounds every
- * sequence's new tokens (at most 1024; a sequence with more is skipped with
- * NCM_ERANGE) and heads / kv_heads is at most 64. Scores, softmax and sums are f32; the
- * probabilities are rounded to bf16 for their product with the values. The
+ * 16-byte aligned, the two ranges apart), lse [rows, heads] f32 or NULL. max_nodes
+ * bounds every sequence's new tokens (at most 1024; a sequence with more is skipped
+ * with NCM_ERANGE), heads / kv_heads is at most 64 and max_nodes * heads /
+ * kv_heads at most 32768. Scores (taken to be above -1e30), softmax and sums are
+ * f32; for their product with the values the probabilities are rounded to bf16,
+ * or, over codes and up to 64 rows of a kv head, to f16 (the values' scales, not
+ * negative, included). A new token's key or value that is not finite reaches only
+ * the nodes that see it. The
  * result does not depend on how the keys are split over the GPU beyond f32 rounding,
  * and is the same on every run. `workspace` (16-byte aligned device memory) of
  * ncm_tree_attention_workspace bytes carries partial sums within the call. */
@@ -644,16 +650,18 @@ NCM_API int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, cons
 /* Rules on next-token logits, all optional (NULL). Row r owns tokens
  * token_start[r] .. token_start[r + 1] of `tokens` (num_tokens entries): its prompt (the
  * first prompt_lens[r]; NULL: none) and what it produced since. In this order:
- *   repetition[r] (> 0): logits of tokens seen at all: l > 0 ? l / rep : l * rep
+ *   repetition[r] (> 0): logits of tokens seen at all: l > 0 ? l * (1 / rep) : l * rep
  *   frequency[r], presence[r]: l -= frequency * count + presence * [count > 0],
  *     count = how often the token was produced (the prompt does not count)
  *   bias entries bias_start[r] .. bias_start[r + 1] of bias_ids / bias
- *     (num_bias entries): l += bias; a repeated id adds each of its entries in order
+ *     (num_bias entries): l += bias; a repeated id adds each of its entries in
+ *     order (which takes a search of the row's later entries)
  *   allowed: bit masks [allowed_count, ceil(vocab / 32)] with row stride
  *     allowed_stride words; row r uses mask allowed_rows[r] (NULL: mask r;
  *     -1: none); a token whose bit is 0 becomes -inf, whatever it was.
  * A token id outside [0, vocab), or list bounds or a mask row outside their
- * array, is ignored and makes ncm_sync report NCM_ERANGE. */
+ * array, is ignored and makes ncm_sync report NCM_ERANGE. num_tokens and num_bias
+ * are at most 2^30. */
 typedef struct ncm_logit_rules {
   const int32_t* tokens;
   const int32_t* token_start; /* [rows + 1] */
@@ -675,8 +683,8 @@ typedef struct ncm_logit_rules {
 /* out = the rules applied to logits [rows, vocab] (NCM_DTYPE_F32 or
  * NCM_DTYPE_BF16, row strides in elements), computed in f32. out_dtype is
  * NCM_DTYPE_F32, or NCM_DTYPE_BF16 for bf16 logits. out may be logits (same type and
- * stride: in place); other overlaps are refused. Rows are what
- * ncm_tied_head_logits or a language-model head wrote. */
+ * stride: in place); other overlaps are refused. At most 65535 rows. Rows are
+ * what ncm_tied_head_logits or a language-model head wrote. */
 NCM_API int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dtype, int64_t stride, void* out,
                                int32_t out_dtype, int64_t out_stride, int64_t rows, int64_t vocab,
                                const ncm_logit_rules_t* rules, ncm_stream_t stream);

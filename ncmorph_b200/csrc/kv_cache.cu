@@ -153,9 +153,8 @@ __device__ __forceinline__ int slot_of_row(const RowsArgs& a, long long t) {
   } else {
     begin = a.begin != nullptr ? __ldg(a.begin + b) : 0;
   }
-  const long long cap = static_cast<long long>(a.batch.table_width) << a.pools.page_shift;
   // a sequence that does not fit is skipped as a whole
-  if (first < 0 || begin < 0 || static_cast<long long>(begin) + n > cap ||
+  if (first < 0 || begin < 0 || static_cast<long long>(begin) + n > kv_capacity(a.batch, a.pools) ||
       static_cast<long long>(first) + n > a.batch.rows) {
     atomicOr(a.err, kErrBadIndex);
     return -1;
@@ -209,7 +208,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
       x[k] = make_uint4(0u, 0u, 0u, 0u);
       if (at[k] < 0) continue;
       if constexpr (APPEND) {
-        x[k] = *reinterpret_cast<const uint4*>(rows + i * stride);
+        x[k] = __ldcs(reinterpret_cast<const uint4*>(rows + i * stride));
       } else if constexpr (CODES) {
         const uint2 c = *reinterpret_cast<const uint2*>(codes + at[k] * HD);
         x[k].x = c.x;

@@ -97,6 +97,12 @@ __device__ __forceinline__ int sequence_of_row(const int32_t* token_start, int b
   return lo;
 }
 
+// Keys that a sequence has at most: what its row of the page table covers, and
+// 2^30, so that a position plus a tile stays in 32 bits.
+__device__ __forceinline__ int kv_capacity(const KvBatch& b, const KvPools& c) {
+  return static_cast<int>(min(static_cast<long long>(b.table_width) << c.page_shift, 1ll << 30));
+}
+
 // Element offset of slot `off` of page `page`, head `h`, in units of rows.
 __device__ __forceinline__ long long kv_slot(const KvPools& c, int page, int h, int off) {
   return ((static_cast<long long>(page) * c.kv_heads + h) << c.page_shift) + off;

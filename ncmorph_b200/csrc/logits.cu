@@ -23,6 +23,7 @@ namespace ncm {
 namespace {
 
 constexpr int kMaxThreads = 512;
+constexpr int64_t kMaxEntries = 1 << 30;  // of a list: a place plus a block's stride stays in 32 bits
 constexpr uint32_t kInPrompt = 0x80000000u;
 // A token's bias entries: 0 none; otherwise 2^31 - 1 minus the first one's place
 // (larger is earlier), and this bit where there are more.
@@ -269,12 +270,12 @@ extern "C" int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dt
                     (long long)vocab, (long long)stride, (long long)out_stride);
   const size_t isz = dtype == NCM_DTYPE_F32 ? 4 : 2, osz = out_dtype == NCM_DTYPE_F32 ? 4 : 2;
   const ncm_logit_rules_t& r = *rules;
-  if (r.tokens != nullptr && (r.token_start == nullptr || r.num_tokens < 0 || r.num_tokens > INT32_MAX))
-    return ncm_fail(NCM_EINVAL, "logits_process: tokens need token_start and num_tokens");
+  if (r.tokens != nullptr && (r.token_start == nullptr || r.num_tokens < 0 || r.num_tokens > kMaxEntries))
+    return ncm_fail(NCM_EINVAL, "logits_process: tokens need token_start and num_tokens (at most 2^30)");
   if (r.tokens == nullptr && (r.repetition || r.frequency || r.presence))
     return ncm_fail(NCM_EINVAL, "logits_process: penalties need tokens");
-  if (r.bias != nullptr && (!r.bias_ids || !r.bias_start || r.num_bias < 0 || r.num_bias > INT32_MAX))
-    return ncm_fail(NCM_EINVAL, "logits_process: bias needs bias_ids, bias_start and num_bias");
+  if (r.bias != nullptr && (!r.bias_ids || !r.bias_start || r.num_bias < 0 || r.num_bias > kMaxEntries))
+    return ncm_fail(NCM_EINVAL, "logits_process: bias needs bias_ids, bias_start and num_bias (at most 2^30)");
   const int64_t words = (vocab + 31) / 32;
   if (r.allowed != nullptr && (r.allowed_count < 0 || r.allowed_stride < words ||
                                r.allowed_stride > INT64_MAX / 8 / (r.allowed_count + 1)))

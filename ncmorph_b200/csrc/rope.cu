@@ -46,7 +46,7 @@ template <bool VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int BATCH = 4;
+  constexpr int BATCH = 2;
   constexpr bool TWO = !INTERLEAVED || !VEC;  // a unit is two loads
   constexpr int PAIRS = VEC ? (INTERLEAVED ? 4 : 8) : 1;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
       if (k0 + k >= n) break;
       const uint16_t* p = src + k * a.x_stride;
       if constexpr (VEC) {
-        v[k] = *reinterpret_cast<const uint4*>(p);
-        if (TWO && rot) z[k] = *reinterpret_cast<const uint4*>(p + step);
+        v[k] = __ldcs(reinterpret_cast<const uint4*>(p));
+        if (TWO && rot) z[k] = __ldcs(reinterpret_cast<const uint4*>(p + step));
       } else {
         v[k].x = *p;
         if (rot) z[k].x = p[step];
@@ -126,11 +126,11 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
             f[x] = pack_rn_bf16x2(q0, q1);
           }
           v[k] = make_uint4(e[0], e[1], e[2], e[3]);
-          *reinterpret_cast<uint4*>(q + step) = make_uint4(f[0], f[1], f[2], f[3]);
+          __stcs(reinterpret_cast<uint4*>(q + step), make_uint4(f[0], f[1], f[2], f[3]));
         }
       }
       if constexpr (VEC)
-        *reinterpret_cast<uint4*>(q) = v[k];
+        __stcs(reinterpret_cast<uint4*>(q), v[k]);
       else
         *q = static_cast<uint16_t>(v[k].x);
     }

@@ -43,7 +43,6 @@ namespace {
 
 constexpr int kTile = 32;  // keys of one ring stage
 
-
 // c += A B, m16n8k16; HALF: f16 operands, otherwise bf16.
 template <bool HALF>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -742,9 +741,13 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
     resident[index].store(std::max(1, n));
     ready[index].set(ctx->device);
   }
-  const int64_t cap = static_cast<int64_t>(batch->table_width) * cache->page_size;
+  const int64_t cap = std::min<int64_t>(static_cast<int64_t>(batch->table_width) * cache->page_size, 1 << 30);
   p->merge = cap > kWholeKeys;
   p->unit_keys = p->merge ? kUnitKeys : static_cast<int>(kWholeKeys);
+  const int64_t tiles = ceil_div(static_cast<int64_t>(max_nodes) * (heads / cache->kv_heads), p->v.rows);
+  // (the kernels multiply the number of units by that of the CTAs)
+  if (batch->batch * cache->kv_heads * tiles * ceil_div(cap, p->unit_keys) > INT64_MAX / (2 * kMaxParts))
+    return ncm_fail(NCM_EINVAL, "%s: too many keys", what);
   p->grid = std::min(kMaxParts, ctx->num_sms * resident[index].load());
   p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
   return NCM_OK;

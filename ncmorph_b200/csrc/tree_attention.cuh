@@ -103,7 +103,7 @@ __device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, bool report) {
   s.len = __ldg(a.batch.kv_lens + b);
   const bool bad = s.first < 0 || s.n < 0 || s.n > a.max_nodes || s.len < s.n ||
                    static_cast<long long>(s.first) + s.n > a.batch.rows ||
-                   s.len > (static_cast<long long>(a.batch.table_width) << a.pools.page_shift);
+                   s.len > kv_capacity(a.batch, a.pools);
   if (bad) {
     if (report) atomicOr(a.err, kErrBadIndex);
     s.n = s.len = 0;

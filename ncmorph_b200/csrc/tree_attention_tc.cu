@@ -527,11 +527,10 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
           ++jo;
         }
       }
-      if (!ok) {
-        fail();
-        tc_commit(&B.drain[g]);
-        mbar_wait(&B.drain[g], 0, nullptr);
-      }
+      if (!ok) fail();
+      // nothing of this group's is on its way to shared or tensor memory once this arrives
+      tc_commit(&B.drain[g]);
+      mbar_wait(&B.drain[g], 0, nullptr);
     }
   } else {
     // ------------------------------------------------------------------ loads

@@ -139,6 +139,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     zeros and -inf."""
     dev, hd = cache.device, cache.head_dim
     if heads is None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] % hd:
+            raise ValueError(f"q must be a matrix of heads of {hd} columns")
         heads = q.shape[1] // hd
     width = heads * hd
     qs = need_rows(q, bf16, "q", dev, width)
@@ -146,7 +148,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     b = _batch(cache, token_start, kv_lens, page_table, T)
     words = 0
     if tree_mask is not None:
-        if tree_mask.dim() != 2 or tree_mask.dtype != i32 or tree_mask.device != dev or tree_mask.shape[0] != T or \
+        if not isinstance(tree_mask, torch.Tensor) or tree_mask.dim() != 2 or tree_mask.dtype != i32 or tree_mask.device != dev or tree_mask.shape[0] != T or \
                 not tree_mask.is_contiguous():
             raise ValueError(f"tree_mask must be a contiguous int32 [{T}, words] tensor on {dev}")
         words = tree_mask.shape[1]

@@ -854,3 +854,179 @@ def test_empty_calls(cuda_dev):
     none = torch.zeros((0, 4), dtype=torch.int32, device=cuda_dev)
     kv_cache.append(cache, bf(2, 128), bf(2, 128), i32(0), i32(), none)
     assert ncm_model.process_logits(torch.zeros((0, 9), device=cuda_dev)).shape == (0, 9)
+
+
+# ------------------------------------------------- limits, and calls at the same time
+
+def test_positions_past_the_limit_are_reported(cuda_dev):
+    """Positions that pass 2^30 or 32 bits although the page table would cover them."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, torch.bfloat16, [40], [2], 1, 64, 1024, slack=1).fill()
+    i32 = lambda *z: torch.tensor(z, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    wide = torch.zeros((1, (1 << 21) + 8), dtype=torch.int32, device=cuda_dev)  # 2^31 + 8192 positions
+    before = w.cache.k.clone()  # (holds NaN where nothing was written: compared as bits)
+    rows = torch.ones((8, 64), device=cuda_dev).to(torch.bfloat16)
+    for begin in (2 ** 31 - 4, 2 ** 30 - 4):
+        out = torch.full((8, 64), 3.0, device=cuda_dev).to(torch.bfloat16)
+        kv_cache.gather(w.cache, i32(0, 8), wide, begin=i32(begin), out_k=out, out_v=out.clone())
+        expect_range_error(cuda_dev)
+        assert torch.all(out == 3.0)
+    for length in (2 ** 31 - 1, 2 ** 30 + 1):
+        kv_cache.append(w.cache, rows, rows, i32(0, 8), i32(length), wide)
+        expect_range_error(cuda_dev)
+        assert torch.equal(w.cache.k.view(torch.int16), before.view(torch.int16))
+        for n in (8, 512):  # (both attention kernels)
+            out = torch.full((8, 64), 3.0, device=cuda_dev).to(torch.bfloat16)
+            kv_cache.tree_attention(rows, w.cache, i32(0, 8), i32(length), wide, max_nodes=n, out=out)
+            expect_range_error(cuda_dev)
+            assert torch.all(out == 3.0)
+    # the last position that the limit allows
+    k, _ = kv_cache.gather(w.cache, i32(0, 8), wide, rows=8, begin=i32(2 ** 30 - 8))
+    assert torch.equal(k.view(torch.int16), before[0, 0, 1016:].view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("page", [8, 1024])
+@pytest.mark.parametrize("n,heads,hd", [(1, 64, 64), (1, 64, 128), (2, 4, 64), (100, 2, 128), (200, 2, 64)])
+def test_smallest_and_largest_pages_and_groups(cuda_dev, dtype, page, n, heads, hd):
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, dtype, [1500, 200 + n], [n, n], 1, hd, page).fill()
+    q = torch.randn((2 * n, heads * hd), generator=w.g).to(torch.bfloat16)
+    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=n, return_lse=True)
+    check_attention(out, lse, attend_ref(w, q, heads, None, hd ** -0.5))
+
+
+def test_most_nodes(cuda_dev):
+    """1024 drafted tokens in one sequence beside one in another, with masks of 32 words."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, torch.bfloat16, [1300, 40], [1024, 1], 1, 64, 16).fill()
+    sees, bits = tree_masks(w.new, w.g)
+    assert bits.shape[1] == 32
+    q = torch.randn((1025, 2 * 64), generator=w.g).to(torch.bfloat16)
+    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=1024,
+                                       tree_mask=bits.to(cuda_dev), return_lse=True)
+    check_attention(out, lse, attend_ref(w, q, 2, sees, 0.125))
+
+
+def test_sequences_that_share_pages(cuda_dev):
+    """Two sequences over the same prefix pages answer as each would alone."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, torch.int8, [200], [1], 2, 64, 16).fill()
+    q = torch.randn((1, 8 * 64), generator=w.g).to(torch.bfloat16).to(cuda_dev)
+    i32 = lambda *z: torch.tensor(z, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    call = lambda q, lens: kv_cache.tree_attention(q, w.cache, i32(*range(len(lens) + 1)), i32(*lens),  # noqa: E731
+                                                   w.table.expand(len(lens), -1).contiguous(), max_nodes=1)
+    both = call(torch.cat([q, q, q]), [200, 90, 200])
+    assert torch.equal(both[0], both[2])
+    for i, n in ((0, 200), (1, 90)):
+        o = call(q, [n])[0].float()  # (another split of the keys)
+        assert torch.all((both[i].float() - o).abs() <= 2 * BF * o.abs() + 2 * BF)
+
+
+def test_two_streams_and_two_graphs_at_once(cuda_dev):
+    """Calls that run at the same time share nothing; a graph may be captured
+    without any call before it."""
+    from ncmorph_b200 import kv_cache, ncm_model
+    cos, sin = tables(4096, 128, cuda_dev)
+    jobs = []
+    for seed, dtype, n in ((1, torch.float8_e4m3fn, 3), (2, torch.float8_e4m3fn, 40), (3, torch.int8, 70)):
+        w = World(cuda_dev, dtype, [3000, 900, 80], [n, n, n], 2, 128, 32, seed=seed).fill()
+        x = torch.randn((3 * n, 8 * 128), generator=w.g).to(torch.bfloat16).to(cuda_dev)
+        pos = torch.arange(3 * n, dtype=torch.int32, device=cuda_dev)
+        hist = torch.randint(0, 1024, (500,), generator=w.g).to(torch.int32).to(cuda_dev)
+        at = torch.linspace(0, 500, 3 * n + 1).int().to(cuda_dev)
+        rep = torch.full((3 * n,), 1.5, device=cuda_dev)
+
+        def run(w=w, x=x, pos=pos, hist=hist, at=at, rep=rep, n=n):
+            q = ncm_model.rope_bf16(x, pos, cos, sin, 8, 128)
+            out, lse = kv_cache.tree_attention(q, w.cache, w.start, w.kv_lens, w.table, max_nodes=n, return_lse=True)
+            return out, lse, ncm_model.process_logits(out, tokens=hist, token_start=at, repetition=rep)
+        jobs.append(run)
+    graphs, outs = [], []
+    for run in jobs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run())
+        graphs.append(graph)
+    want = [run() for run in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        eager = []
+        for run, stream in zip(jobs, streams):
+            with torch.cuda.stream(stream):
+                eager.append(run())
+        torch.cuda.synchronize()
+        for a, b, c in zip(outs, want, eager):
+            assert all(torch.equal(x, y) and torch.equal(z, y) for x, y, z in zip(a, b, c)), turn
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logit_rows_of_any_alignment(cuda_dev, dtype):
+    """Rows that start on odd elements give the bits that aligned rows give."""
+    from ncmorph_b200 import ncm_model
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((3, 3001), generator=g).to(dtype).to(cuda_dev)
+    i32 = lambda *z: torch.tensor(z, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    args = dict(tokens=i32(*range(0, 3000, 7)), token_start=i32(0, 100, 100, 429), presence=torch.ones(3, device=cuda_dev),
+                bias_ids=i32(2999, 3000, 0), bias=torch.ones(3, device=cuda_dev), bias_start=i32(0, 1, 1, 3))
+    want = ncm_model.process_logits(torch.nn.functional.pad(x, (0, 7))[:, :3001], **args)
+    odd = torch.zeros((3, 3013), dtype=dtype, device=cuda_dev)
+    for shift in (1, 2, 3):
+        odd[:, shift:shift + 3001] = x
+        assert torch.equal(ncm_model.process_logits(odd[:, shift:shift + 3001], **args), want)
+
+
+def test_refusals_of_sizes(cuda_dev):
+    import ctypes
+    from ncmorph_b200 import _lib, kv_cache, ncm_model
+    from ncmorph_b200.device import context_of, raw_stream
+    bf = lambda *s: torch.zeros(s, device=cuda_dev, dtype=torch.bfloat16)  # noqa: E731
+    i32 = lambda *z: torch.tensor(z, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    cache = kv_cache.KVCache.allocate(64, 16, 1, 64, torch.bfloat16, cuda_dev)
+    table, start, lens = torch.zeros((1, 64), dtype=torch.int32, device=cuda_dev), i32(0, 1), i32(1)
+    for heads, nodes in ((1, 1025), (65, 1), (64, 513)):
+        with pytest.raises(_lib.NcmError):
+            kv_cache.tree_attention(bf(1, heads * 64), cache, start, lens, table, max_nodes=nodes)
+    with pytest.raises(ValueError):  # a part of a head
+        kv_cache.tree_attention(bf(1, 80), cache, start, lens, table, max_nodes=1)
+    with pytest.raises(ValueError):
+        kv_cache.tree_attention(bf(64), cache, start, lens, table, max_nodes=1)
+    with pytest.raises(ValueError):
+        kv_cache.tree_attention(bf(1, 64), cache, start, lens, table, max_nodes=1, tree_mask=[[1]])
+    with pytest.raises(_lib.NcmError):
+        kv_cache.tree_attention(bf(1, 64), cache, start, lens, table, max_nodes=1, tree_mask=torch.zeros((1, 33), dtype=torch.int32, device=cuda_dev))
+    for shape in ((4, 1, 16, 96), (4, 1, 24, 64), (4, 1, 4, 64), (4, 1, 2048, 64)):
+        odd = kv_cache.KVCache.allocate(*(shape[i] for i in (0, 2, 1, 3)), torch.bfloat16, cuda_dev)
+        with pytest.raises(_lib.NcmError):
+            kv_cache.append(odd, bf(1, shape[3]), bf(1, shape[3]), start, lens, table)
+    # a workspace that is missing or too small
+    q, out = bf(1, 64), bf(1, 64)
+    b = kv_cache._batch(cache, start, lens, table, 1)
+    n = ctypes.c_uint64()
+    _lib.call("ncm_tree_attention_workspace", context_of(cache.device), cache._ref, ctypes.byref(b), 1, 1, ctypes.byref(n))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=cuda_dev)
+    for p, size in ((None, n.value), (ws.data_ptr(), n.value - 1), (ws.data_ptr() + 4, n.value)):
+        with pytest.raises(_lib.NcmError):
+            _lib.call("ncm_tree_attention", context_of(cache.device), cache._ref, ctypes.byref(b), q.data_ptr(), 64, None, 0, 1, 1,
+                      0.125, out.data_ptr(), 64, None, p, size, raw_stream(cache.device))
+    # lists and rows past what the logit rules take
+    x = torch.zeros((1, 32), device=cuda_dev)
+    one = torch.ones(1, device=cuda_dev)
+    for field, value in (("num_tokens", (1 << 30) + 1), ("num_bias", (1 << 30) + 1), ("num_tokens", -1), ("rows", 65536)):
+        r = _lib.LogitRules()
+        r.tokens, r.token_start, r.num_tokens = lens.data_ptr(), start.data_ptr(), 1
+        r.bias_ids, r.bias, r.bias_start, r.num_bias = lens.data_ptr(), one.data_ptr(), start.data_ptr(), 1
+        if field != "rows":
+            setattr(r, field, value)
+        with pytest.raises(_lib.NcmError):
+            _lib.call("ncm_logits_process", context_of(cache.device), x.data_ptr(), ncm_model.LOGIT_TYPES[torch.float32], 32, x.data_ptr(),
+                      ncm_model.LOGIT_TYPES[torch.float32], 32, value if field == "rows" else 1, 32, ctypes.byref(r), raw_stream(cache.device))
