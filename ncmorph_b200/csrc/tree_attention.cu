@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
   const uint32_t ring = smem_u32(smem) + kg * NST * S::kStageBytes;
   pdl_wait();
 
-  Walk<ROWS> w(a, blockIdx.x, a.grid);
+  Walk<ROWS> w(a, blockIdx.x);
   auto group_sync = [&] {
     if constexpr (RG == 1)
       __syncwarp();
@@ -543,61 +543,49 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
   }
 }
 
-// Adds up the partial sums of one row of one item (blockIdx.x: sequence and kv
-// head, blockIdx.y: row of the sequence's rows), in an order that the split
-// alone decides. An item of one long sequence may have a part from every CTA,
-// so the parts' maxima and sums are fetched by one thread each, and their
-// values by 128 / (HD / 4) groups of threads with four loads in flight.
-//
-// What the caller gave is read before the wait: the attention kernel lets this
-// one start only after its own wait, so the kernels in front of it are done.
+// Adds up the partial sums of a row of an item (blockIdx.x: sequence and kv
+// head, blockIdx.y: 4 / WPR rows of the sequence's rows), in an order that the
+// split alone decides. WPR warps share a row: all four of the block where an item
+// of few long sequences has tens of parts, one where it has a few. What the caller
+// gave is read before the wait: the attention kernel does not let this one start
+// ahead of its own end, and the kernels in front of both are done by then.
 constexpr int kMaxParts = 2048;  // CTAs of the attention kernel at most
 
-template <int HD>
+template <int HD, int WPR>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int ROWS) {
-  constexpr int STR = HD + 4, LPP = HD / 4, GROUPS = 128 / LPP;  // lanes of a part, parts at a time
-  __shared__ float weight[kMaxParts];
+  constexpr int STR = HD + 4, LPP = HD / 4, GROUPS = 32 * WPR / LPP;  // lanes of a part, parts at a time
   __shared__ float red[4][3];
-  __shared__ float4 vals[GROUPS][LPP];
+  __shared__ float4 vals[WPR == 4 ? GROUPS : 1][LPP];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x % (32 * WPR);  // of the row's threads
   const int b = blockIdx.x / a.pools.kv_heads, kvh = blockIdx.x - b * a.pools.kv_heads;
   const Seq s = load_seq(a, b, false);
-  const int row_all = blockIdx.y;
-  const bool exists = row_all < s.n * a.group;
+  const int row_all = blockIdx.y * (4 / WPR) + (WPR == 1 ? warp : 0);
   const int tile = row_all / ROWS, row = row_all - tile * ROWS;
-  int c0 = 0, c1 = 0;
-  long long all = 0;
-  if (exists) {
-    auto tiles = [&](const Seq& q) { return (q.n * a.group + ROWS - 1) / ROWS; };
-    const int units = units_of(a, s);
-    long long before = 0;
-    for (int i = lane; i < a.batch.batch; i += 32) {
-      const Seq q = load_seq(a, i, false);
-      const long long u = static_cast<long long>(tiles(q)) * a.pools.kv_heads * units_of(a, q);
-      all += u;
-      if (i < b) before += u;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-    }
-    const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units, x1 = x0 + units - 1;
-    c0 = static_cast<int>(((x0 + 1) * a.grid - 1) / all);
-    c1 = static_cast<int>(((x1 + 1) * a.grid - 1) / all);
+  auto tiles = [&](const Seq& q) { return (q.n * a.group + ROWS - 1) / ROWS; };
+  const int units = units_of(a, s);
+  long long before = 0, total = 0;
+  for (int i = lane; i < a.batch.batch; i += 32) {
+    const Seq q = load_seq(a, i, false);
+    const long long u = static_cast<long long>(tiles(q)) * a.pools.kv_heads * units_of(a, q);
+    total += u;
+    if (i < b) before += u;
   }
+  before = warp_sum(before);
+  total = warp_sum(total);
+  const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units;
+  const Deal deal(a, total);
+  const bool exists = row_all < s.n * a.group;
+  const int c0 = exists ? deal.owner(x0) : 0, c1 = exists ? deal.owner(x0 + units - 1) : 0;
   pdl_wait();
   pdl_launch_dependents();
-  if (c0 == c1) return;  // one CTA had the whole item, and wrote its rows
+  if (c0 == c1) return;  // no such row, or one CTA had the whole item and wrote its rows
   const int n = c1 - c0 + 1;
   const float* first = a.part + row * STR;
   auto part_of = [&](int k) { return first + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * ROWS * STR; };
-  // a grid larger than the number of units has CTAs without any
-  auto empty = [&](int k) { return all < a.grid && all * (c0 + k) / a.grid == all * (c0 + k + 1) / a.grid; };
-  // ---- maxima, then the weights of the parts and the sum
+  // ---- maxima, then the sum with the parts' weights
   float mm = kFirstMax, mv = kFirstMax;
-  for (int k = threadIdx.x; k < n; k += 128) {
-    if (empty(k)) continue;
+  for (int k = tid; k < n; k += 32 * WPR) {
     const float4 h = *reinterpret_cast<const float4*>(part_of(k));
     mm = fmaxf(mm, h.x);
     mv = fmaxf(mv, h.z);
@@ -607,30 +595,29 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int R
     mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
     mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
   }
-  if (lane == 0) {
-    red[warp][0] = mm;
-    red[warp][1] = mv;
-  }
-  __syncthreads();
-  mm = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
-  mv = fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1]));
-  float sum = 0.f;
-  for (int k = threadIdx.x; k < n; k += 128) {
-    float w = 0.f;
-    if (!empty(k)) {
-      const float4 h = *reinterpret_cast<const float4*>(part_of(k));
-      w = ex2(h.z - mv);
-      sum = fmaf(h.y, ex2(h.x - mm), sum);
+  if constexpr (WPR == 4) {
+    if (lane == 0) {
+      red[warp][0] = mm;
+      red[warp][1] = mv;
     }
-    weight[k] = w;
+    __syncthreads();
+    mm = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+    mv = fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1]));
+  }
+  float sum = 0.f;
+  for (int k = tid; k < n; k += 32 * WPR) {
+    const float4 h = *reinterpret_cast<const float4*>(part_of(k));
+    sum = fmaf(h.y, ex2(h.x - mm), sum);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red[warp][2] = sum;
-  __syncthreads();
-  sum = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
-  // ---- values
-  const int g = threadIdx.x / LPP, d = threadIdx.x % LPP;
+  if constexpr (WPR == 4) {
+    if (lane == 0) red[warp][2] = sum;
+    __syncthreads();
+    sum = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
+  }
+  // ---- values, four parts of a group of lanes in flight
+  const int g = tid / LPP, d = tid % LPP;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = g; k0 < n; k0 += 4 * GROUPS) {
     float4 y[4];
@@ -638,28 +625,41 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int R
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = k0 + i * GROUPS;
-      w[i] = k < n ? weight[k] : 0.f;
+      w[i] = kFirstMax;
       y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k < n && !empty(k)) y[i] = *reinterpret_cast<const float4*>(part_of(k) + 4 + 4 * d);
+      if (k < n) {
+        const float* p = part_of(k);
+        w[i] = p[2];
+        y[i] = *reinterpret_cast<const float4*>(p + 4 + 4 * d);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v.x = fmaf(y[i].x, w[i], v.x);
-      v.y = fmaf(y[i].y, w[i], v.y);
-      v.z = fmaf(y[i].z, w[i], v.z);
-      v.w = fmaf(y[i].w, w[i], v.w);
+      const float f = ex2(w[i] - mv);
+      v.x = fmaf(y[i].x, f, v.x);
+      v.y = fmaf(y[i].y, f, v.y);
+      v.z = fmaf(y[i].z, f, v.z);
+      v.w = fmaf(y[i].w, f, v.w);
     }
   }
-  vals[g][d] = v;
-  __syncthreads();
-  if (g != 0) return;
+  if constexpr (WPR == 4) {
+    vals[g][d] = v;
+    __syncthreads();
+    if (g != 0) return;
 #pragma unroll
-  for (int k = 1; k < GROUPS; ++k) {
-    const float4 y = vals[k][d];
-    v.x += y.x;
-    v.y += y.y;
-    v.z += y.z;
-    v.w += y.w;
+    for (int k = 1; k < GROUPS; ++k) {
+      const float4 y = vals[k][d];
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
+    }
+  } else if constexpr (GROUPS == 2) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+    v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+    if (g != 0) return;
   }
   const int i = row_all / a.group, head = kvh * a.group + row_all - i * a.group;
   const long long t = s.first + static_cast<long long>(i);
@@ -709,12 +709,15 @@ Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
 }
 
 // Contexts this short are not split (no second kernel): one unit holds all keys.
-constexpr int64_t kWholeKeys = 512;
-constexpr int kUnitKeys = 128;
+constexpr int kWholeShift = 9;
+constexpr int kUnitShift = 7;
+
+// Parts of an item, on average, that one warp of the merge adds up; more are shared by four.
+constexpr int kFewParts = 8;
 
 struct Plan {
   Variant v;
-  int grid, unit_keys;
+  int grid, unit_shift;
   bool merge;
   uint64_t bytes;
 };
@@ -742,11 +745,11 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
     ready[index].set(ctx->device);
   }
   const int64_t cap = std::min<int64_t>(static_cast<int64_t>(batch->table_width) * cache->page_size, 1 << 30);
-  p->merge = cap > kWholeKeys;
-  p->unit_keys = p->merge ? kUnitKeys : static_cast<int>(kWholeKeys);
+  p->merge = cap > 1 << kWholeShift;
+  p->unit_shift = p->merge ? kUnitShift : kWholeShift;
   const int64_t tiles = ceil_div(static_cast<int64_t>(max_nodes) * (heads / cache->kv_heads), p->v.rows);
   // (the kernels multiply the number of units by that of the CTAs)
-  if (batch->batch * cache->kv_heads * tiles * ceil_div(cap, p->unit_keys) > INT64_MAX / (2 * kMaxParts))
+  if (batch->batch * cache->kv_heads * tiles * ceil_div(cap, 1 << p->unit_shift) > INT64_MAX / (2 * kMaxParts))
     return ncm_fail(NCM_EINVAL, "%s: too many keys", what);
   p->grid = std::min(kMaxParts, ctx->num_sms * resident[index].load());
   p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
@@ -809,7 +812,7 @@ int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv
   a.out_stride = out_stride;
   a.lse = lse;
   a.part = static_cast<float*>(workspace);
-  a.unit_keys = p.unit_keys;
+  a.unit_shift = p.unit_shift;
   a.err = ctx->d_err;
   const int64_t most_rows = static_cast<int64_t>(max_nodes) * a.group;
   const int64_t items = static_cast<int64_t>(batch->batch) * cache->kv_heads * ceil_div(most_rows, p.v.rows);
@@ -821,9 +824,10 @@ int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv
   }
   if (p.merge) {
     Launch _launch(ctx, KID_ATTENTION, st);
-    auto merge = cache->head_dim == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>;
-    NCM_CUDA_TRY(launch_pdl(merge, dim3(batch->batch * cache->kv_heads, static_cast<unsigned>(most_rows)), dim3(128), 0, st, 1, a,
-                            p.v.rows));
+    const bool wide = cache->head_dim == 128, few = kFewParts * items >= p.grid;
+    auto merge = few ? (wide ? tree_merge_kernel<128, 1> : tree_merge_kernel<64, 1>)
+                     : (wide ? tree_merge_kernel<128, 4> : tree_merge_kernel<64, 4>);
+    NCM_CUDA_TRY(launch_pdl(merge, dim3(batch->batch * cache->kv_heads, ceil_div(most_rows, few ? 4 : 1)), dim3(128), 0, st, 1, a, p.v.rows));
   }
   return NCM_OK;
 }

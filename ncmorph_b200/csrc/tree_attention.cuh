@@ -22,7 +22,7 @@ struct TreeArgs {
   long long out_stride;
   float* lse;
   float* part;  // [2 * grid][ROWS][4 + HD]: m, sum of p, m', -, values
-  int unit_keys;
+  int unit_shift;  // log2 of a unit's keys
   int grid;  // CTAs of the attention kernel
   int* err;
 };
@@ -115,49 +115,31 @@ template <int ROWS>
 __device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) {
   return (s.n * a.group + ROWS - 1) / ROWS;
 }
-__device__ __forceinline__ int units_of(const TreeArgs& a, const Seq& s) { return (s.len + a.unit_keys - 1) / a.unit_keys; }
-
-// Units in front of sequence `upto` (whole warps; every lane gets the sum).
-template <int ROWS>
-__device__ __forceinline__ long long units_before(const TreeArgs& a, int upto) {
-  long long sum = 0;
-  for (int b = threadIdx.x & 31; b < upto; b += 32) {
-    const Seq s = load_seq(a, b, false);
-    sum += static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+__device__ __forceinline__ int units_of(const TreeArgs& a, const Seq& s) {
+  return (s.len + (1 << a.unit_shift) - 1) >> a.unit_shift;
 }
 
-// The sequence that holds unit x < total, and the unit's place in it.
-template <int ROWS>
-__device__ __forceinline__ int find_unit(const TreeArgs& a, long long x, long long* inside) {
-  const int lane = threadIdx.x & 31;
-  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
-    long long u = 0;
-    if (b0 + lane < a.batch.batch) {
-      const Seq s = load_seq(a, b0 + lane, false);
-      u = static_cast<long long>(tiles_of<ROWS>(a, s)) * a.pools.kv_heads * units_of(a, s);
-    }
-    long long before = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += y;
-    }
-    const long long all = __shfl_sync(0xffffffffu, before, 31);
-    before -= u;
-    if (x < all) {
-      const unsigned hit = __ballot_sync(0xffffffffu, x >= before && x < before + u);
-      const int who = __ffs(hit) - 1;
-      *inside = x - __shfl_sync(0xffffffffu, before, who);
-      return b0 + who;
-    }
-    x -= all;
+// x / d for x >= 0, d > 0; in 32 bits where that does, which takes a tenth of the time.
+__device__ __forceinline__ long long quotient(long long x, long long d) {
+  if (((x | d) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(d);
+  return x / d;
+}
+// How `total` units are dealt out: every CTA has `each` consecutive ones, the first `more` one beyond.
+struct Deal {
+  long long each;
+  int more;
+  __device__ __forceinline__ Deal(const TreeArgs& a, long long total)
+      : each(quotient(total, a.grid)), more(static_cast<int>(total - each * a.grid)) {}
+  __device__ __forceinline__ long long first(int cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ int owner(long long unit) const {
+    const long long longer = more * (each + 1);
+    return static_cast<int>(unit < longer ? quotient(unit, each + 1) : more + quotient(unit - longer, each));
   }
-  *inside = 0;
-  return a.batch.batch;
+};
+__device__ __forceinline__ long long warp_sum(long long x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
 // Bits [j0, j0 + 32) of a node's mask row (bits in front of 0 are ones, behind the row zeros).
@@ -184,16 +166,47 @@ struct Walk {
   int kvh, row0, live_rows;  // (live_rows: rows of the item from row0 on; may be more than ROWS)
   int ctx, key0, key1;
 
-  // Whole warps; block 0 of `blocks` reports sequences that do not fit.
-  __device__ __forceinline__ Walk(const TreeArgs& a, int block, int blocks) {
-    const long long total = units_before<ROWS>(a, a.batch.batch);
-    at = total * block / blocks;
-    hi = total * (block + 1) / blocks;
-    if (block == 0 && threadIdx.x < 32)
-      for (int i = threadIdx.x; i < a.batch.batch; i += 32) load_seq(a, i, true);
+  // Whole warps; block 0 reports sequences that do not fit.
+  __device__ __forceinline__ Walk(const TreeArgs& a, int block) {
+    const int lane = threadIdx.x & 31;
+    auto units_at = [&](int i, bool report) {
+      if (i >= a.batch.batch) return 0ll;
+      const Seq q = load_seq(a, i, report);
+      return static_cast<long long>(tiles_of<ROWS>(a, q)) * a.pools.kv_heads * units_of(a, q);
+    };
+    const bool report = block == 0 && threadIdx.x < 32;
+    const long long mine = units_at(lane, report);  // (of the first 32 sequences, which are mostly all)
+    long long total = mine;
+    for (int i = lane + 32; i < a.batch.batch; i += 32) total += units_at(i, report);
+    total = warp_sum(total);
+    const Deal deal(a, total);
+    at = deal.first(block);
+    hi = deal.first(block + 1);
     inside = 0;
-    b = at < hi ? find_unit<ROWS>(a, at, &inside) : a.batch.batch;
     u0 = u1 = 0;
+    b = a.batch.batch;
+    if (at >= hi) return;
+    // the sequence that holds unit `at`
+    long long x = at;
+    for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
+      const long long u = b0 == 0 ? mine : units_at(b0 + lane, false);
+      long long before = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      const long long all = __shfl_sync(0xffffffffu, before, 31);
+      before -= u;
+      if (x < all) {
+        const unsigned hit = __ballot_sync(0xffffffffu, x >= before && x < before + u);
+        const int who = __ffs(hit) - 1;
+        inside = x - __shfl_sync(0xffffffffu, before, who);
+        b = b0 + who;
+        break;
+      }
+      x -= all;
+    }
   }
   __device__ __forceinline__ bool next(const TreeArgs& a) {
     at += u1 - u0;
@@ -208,15 +221,15 @@ struct Walk {
         inside = 0;
         continue;
       }
-      const int item = static_cast<int>(inside / units);
+      const int item = static_cast<int>(quotient(inside, units));
       u0 = static_cast<int>(inside - static_cast<long long>(item) * units);
       u1 = static_cast<int>(min(static_cast<long long>(units), u0 + (hi - at)));
       kvh = item / tiles;
       row0 = (item - kvh * tiles) * ROWS;
       live_rows = s.n * a.group - row0;
       ctx = s.len - s.n;
-      key0 = u0 * a.unit_keys;
-      key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) * a.unit_keys));
+      key0 = u0 << a.unit_shift;
+      key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) << a.unit_shift));
       return true;
     }
     return false;

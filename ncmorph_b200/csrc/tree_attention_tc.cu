@@ -37,14 +37,13 @@ struct TcBars {
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
   uint64_t s_full[2][2], s_free[2][2];  // [group][buffer]
   uint64_t p_full[2][2], pv_done[2][2];
-  uint64_t sums_full[4], cols_full[4][2], cols_free[4][2];  // [warp pair] the second group's sums, and 32 columns of its values
+  uint64_t sums_full[4], taken[4];  // [pair of the groups' warps] their sums are there; both have read both groups' values
   uint64_t drain[2];
   uint32_t tmem_base;
   int abort_flag;
-  float2 sums[128];  // the second group's maxima and sums
   int odd_values;  // a loader met a value that is not finite in a tile of new tokens
 };
-constexpr int kBarBytes = 2048;
+constexpr int kBarBytes = 512;
 static_assert(sizeof(TcBars) <= kBarBytes, "barriers");
 
 // SPLITQ: the groups have 128 rows each; otherwise the same 128 rows and every other tile.
@@ -90,7 +89,8 @@ struct TcShape {
   static constexpr bool kRawScales = kCodes && !kInRegs;
   static constexpr int kRawScale = kScale + (kCodes ? kScaleSlots * 2 * kBK * 4 : 0);  // [raw][K, V][kBK] f32
   static constexpr int kBars = kRawScale + (kRawScales ? kRaw * 2 * kBK * 4 : 0);
-  static constexpr int kSmem = kBars + kBarBytes + 1024;  // (1024: the base is aligned up)
+  static constexpr int kSums = kBars + kBarBytes;  // !SPLITQ: the groups' maxima and sums, [group][128]
+  static constexpr int kSmem = kSums + (SPLITQ ? 0 : 2 * 128 * 8);
   static constexpr uint32_t kTmemCols = 512;  // S: 2 x 2 x 64, O: 2 x head_dim
   static_assert(kSmem <= 232448, "shared memory of the tcgen05 attention");
 };
@@ -149,8 +149,11 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
   using S = TcShape<HD, FMT, SPLITQ>;
   constexpr bool CODES = S::kCodes;
   constexpr int BK = S::kBK, RB = S::kRowBytes, CPR = RB / 16, NS = S::kStages, LG = S::kLoadGroups, NB = S::kBlocks, ROWS = S::kRows;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0u) {  // (there is no room to align it by hand)
+    if (threadIdx.x == 0) atomicOr(a.err, kErrWaitTimeout);
+    return;
+  }
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -169,11 +172,8 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         mbar_init(&B.pv_done[g][i], 1);
       }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&B.sums_full[i], 1);
-      for (int x = 0; x < 2; ++x) {
-        mbar_init(&B.cols_full[i][x], 1);
-        mbar_init(&B.cols_free[i][x], 1);
-      }
+      mbar_init(&B.sums_full[i], 2);
+      mbar_init(&B.taken[i], 2);
     }
     mbar_init(&B.drain[0], 1);
     mbar_init(&B.drain[1], 1);
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
     if (lane == 0) done = tc_wait(bar, parity, abort_flag);
     return __shfl_sync(0xffffffffu, done, 0) != 0;
   };
-  Walk<ROWS> w(a, blockIdx.x, a.grid);
+  Walk<ROWS> w(a, blockIdx.x);
   uint32_t number = 0;  // of the segment's first tile: they are numbered over all segments
 
   if (warp < 8) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
     constexpr int STEP = SPLITQ ? 1 : 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t obase = tmem + lanes + 256 + g * HD;
-    uint32_t j = 0, segment = 0, rounds = 0;  // tiles, segments and sums handed over so far
+    uint32_t j = 0, segment = 0, joined = 0;  // tiles, segments, and those whose sums were joined so far
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // (uniform over the warp)
       ok = warp_wait(bar, parity);
@@ -376,59 +376,54 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       if (!ok) break;
       if (!busy) continue;
       tc_fence_after();
-      // ---- this row's sums: out, or its part of them; the second group's go to the
-      // first through its own P buffers, [32 columns][128 rows] at a time, in XB buffers
+      // ---- this row's sums: out, or its part of them. Where the groups had the same
+      // rows, a row's values lie in the same lane of tensor memory: each group adds
+      // up half of the columns.
       const bool whole = w.whole();
       const bool odd = !CODES && *const_cast<volatile int*>(&B.odd_values) != 0;
-      constexpr uint32_t XB = S::kPBufs * S::kPBytes / 16384;
-      float f0 = 1.f, f1 = 0.f;  // weights of the groups' values
+      constexpr int COLS = SPLITQ ? HD : HD / 2;
+      const int d0 = SPLITQ ? 0 : g * COLS;
+      float f0 = 1.f, f1 = 0.f;  // weights of this group's and the other one's values
+      bool two = false;
       if constexpr (!SPLITQ) {
-        if (g == 1) {
-          B.sums[row] = make_float2(m, l);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B.sums_full[warp & 3]);
-        } else {
-          if (!wait(&B.sums_full[warp & 3], (rounds / (HD / 32)) & 1u)) break;
-          const float2 other = B.sums[row];
-          const float to = fmaxf(m, other.x);
-          f0 = ex2(m - to);
-          f1 = ex2(other.x - to);
-          l = l * f0 + other.y * f1;
-          m = to;
-        }
+        float2* sums = reinterpret_cast<float2*>(smem + S::kSums) + row;
+        sums[128 * g] = make_float2(m, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.sums_full[warp & 3]);
+        if (!wait(&B.sums_full[warp & 3], joined & 1u)) break;
+        tc_fence_after();
+        const float2 x = sums[0], y = sums[128];
+        m = fmaxf(x.x, y.x);
+        f0 = ex2(x.x - m);
+        f1 = ex2(y.x - m);
+        l = fmaf(x.y, f0, y.y * f1);
+        two = ntiles > 1;  // (otherwise the second group had nothing)
       }
       float* part = a.part + ((2ll * blockIdx.x + (w.u0 == 0 ? 1 : 0)) * ROWS + qt * 128 + row) * (HD + 4);
       uint16_t* out = a.out + token * a.out_stride + head * HD;
+      const uint32_t o0 = SPLITQ ? obase : tmem + lanes + 256;
+      // Rows are turned around in this warp's own piece of P, so that eight lanes store
+      // 32 neighbouring columns of a row.
+      const uint32_t turn = smem_u32(smem + S::kP) + g * S::kPBufs * S::kPBytes + (warp & 3) * 4096;
+      const int rest = live - (warp & 3) * 32;  // rows of this warp
 #pragma unroll 1
-      for (int d = 0; d < HD; d += 32, ++rounds) {
+      for (int d = d0; d < d0 + COLS; d += 32) {
         uint32_t raw[32];
         float* o = reinterpret_cast<float*>(raw);
-        if (any) {
-          tmem_ld_x32(obase + d, raw);
-          tmem_wait_ld();
-        } else {
+        tmem_ld_x32(o0 + d, raw);
+        tmem_wait_ld();
+        if (two) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
-        if constexpr (!SPLITQ) {
-          const uint32_t x = rounds % XB, parity = (rounds / XB) & 1u;
-          float* xch = reinterpret_cast<float*>(smem + S::kP + S::kPBufs * S::kPBytes + x * 16384) + row;
-          if (g == 1) {
-            if (!wait(&B.cols_free[warp & 3][x], parity ^ 1u)) break;
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t more[16];
+            tmem_ld_x16(o0 + HD + d + h, more);
+            tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) xch[i * 128] = o[i];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.cols_full[warp & 3][x]);
-            continue;
+            for (int i = 0; i < 16; ++i) o[h + i] = o[h + i] * f0 + __uint_as_float(more[i]) * f1;
           }
-          if (!wait(&B.cols_full[warp & 3][x], parity)) break;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + xch[i * 128] * f1;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B.cols_free[warp & 3][x]);
         }
-        if (!exists) continue;
-        if (odd) {
+        if (odd && exists) {
           // (the keys of the tiles with new tokens)
           for (int k = w.key0 + (max(w.ctx - w.key0, 0) & ~(BK - 1)); k < w.key1; ++k) {
             const int n2 = k - w.ctx;
@@ -442,34 +437,41 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
               if ((v[i] & 0x7F80u) == 0x7F80u) o[i] += bf16_to_f32(v[i]);
           }
         }
-        if (whole) {
-          const float f = out_factor(l, 0.f);
+        const float f = whole ? out_factor(l, 0.f) : 1.f;
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(out + d + i) =
-                make_uint4(pack_rn_bf16x2(o[i] * f, o[i + 1] * f), pack_rn_bf16x2(o[i + 2] * f, o[i + 3] * f),
-                           pack_rn_bf16x2(o[i + 4] * f, o[i + 5] * f), pack_rn_bf16x2(o[i + 6] * f, o[i + 7] * f));
-        } else {
+        for (int c = 0; c < 8; ++c)
+          sts128(turn + lane * 128 + ((c ^ (lane & 7)) << 4),
+                 make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f), __float_as_uint(o[4 * c + 2] * f),
+                            __float_as_uint(o[4 * c + 3] * f)));
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part + 4 + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3), c = lane & 7;
+          const uint4 x = lds128(turn + r * 128 + ((c ^ (r & 7)) << 4));
+          uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), r));
+          if (r >= rest) continue;
+          if (whole)
+            *reinterpret_cast<uint2*>(to + d + 4 * c) = make_uint2(pack_rn_bf16x2(__uint_as_float(x.x), __uint_as_float(x.y)),
+                                                                   pack_rn_bf16x2(__uint_as_float(x.z), __uint_as_float(x.w)));
+          else
+            *reinterpret_cast<uint4*>(part + (r - lane) * (HD + 4) + 4 + d + 4 * c) = x;
         }
       }
-      if (!ok) break;
       if (exists && (SPLITQ || g == 0)) {
         if (!whole)
           *reinterpret_cast<float4*>(part) = make_float4(m, l, m, 0.f);
         else if (a.lse != nullptr)
           a.lse[token * a.heads + head] = lse_of(m, l);
       }
-      // the last columns must be taken before the second group's P buffers are written
-      // again (which also keeps the pair within one segment: sums has one place)
-      if (!SPLITQ && g == 1) {
-#pragma unroll
-        for (uint32_t x = 0; x < XB; ++x)
-          if (!wait(&B.cols_free[warp & 3][x], ((rounds / XB) & 1u) ^ 1u)) break;
-        if (!ok) break;
-      }
       tc_fence_before();
+      __syncwarp();
+      if constexpr (!SPLITQ) {
+        // neither group's values nor its sums are overwritten before both have read them
+        if (lane == 0) mbar_arrive(&B.taken[warp & 3]);
+        if (!wait(&B.taken[warp & 3], joined & 1u)) break;
+        ++joined;
+      }
     }
     if (!ok) fail();
   } else if (warp < 10) {
@@ -621,7 +623,10 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         }
         const uint32_t from = smem_u32(smem + S::kRawAt) + (n % (S::kRaw + !S::kRaw)) * 2 * BK * RB + tid * 16;
         const uint32_t to = smem_u32(smem + S::kK) + (st * NB + (my_c >> 2)) * S::kBlock + my_key * 128;
-        const uint32_t to0 = (((2 * my_c) & 7) ^ (my_key & 7)) << 4, to1 = (((2 * my_c + 1) & 7) ^ (my_key & 7)) << 4;
+        // (128-wide rows: half of the lanes store their second eight values first, so that a
+        // row's pieces in both 64-dim columns lie in different banks)
+        const uint32_t flip = HD == 128 ? my_c >> 2 & 1 : 0;
+        const uint32_t to0 = (((2 * my_c + flip) & 7) ^ (my_key & 7)) << 4, to1 = to0 ^ 16u;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (n >= NS && !warp_wait(kv ? &B.v_empty[st] : &B.k_empty[st], ((n / NS) - 1) & 1u)) return false;
@@ -632,7 +637,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
               v = held[2 * x + kv];
             else
               v = lds128(from + kv * BK * RB + x * kLoadThreads * 16);
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            const uint32_t e[4] = {flip ? v.z : v.x, flip ? v.w : v.y, flip ? v.x : v.z, flip ? v.y : v.w};
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
