@@ -567,13 +567,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int R
   long long before = 0, total = 0;
   for (int i = lane; i < a.batch.batch; i += 32) {
     const Seq q = load_seq(a, i, false);
-    const long long u = static_cast<long long>(tiles(q)) * a.pools.kv_heads * units_of(a, q);
+    const long long u = places_of(a, q, tiles(q));
     total += u;
     if (i < b) before += u;
   }
   before = warp_sum(before);
   total = warp_sum(total);
-  const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * units;
+  const long long x0 = before + (static_cast<long long>(kvh) * tiles(s) + tile) * (a.begin_cost + units) + a.begin_cost;
   const Deal deal(a, total);
   const bool exists = row_all < s.n * a.group;
   const int c0 = exists ? deal.owner(x0) : 0, c1 = exists ? deal.owner(x0 + units - 1) : 0;
@@ -711,6 +711,11 @@ Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
 // Contexts this short are not split (no second kernel): one unit holds all keys.
 constexpr int kWholeShift = 9;
 constexpr int kUnitShift = 7;
+// What beginning an item costs (query rows, the first keys' way, the sums' way out), in
+// units. us at 0, 2, 3 and 4, eight to 32 sequences of 1 to 16 thousand tokens: one token,
+// bf16, head_dim 64: 39.1, 37.5, 36.8, 37.0; eight, int8: 43.1, 37.8, 33.7, 33.0; 26
+// (tcgen05), e4m3, head_dim 128: 73, 58.0, 55.8, 55.9; one long sequence: no difference.
+constexpr int kBeginCost = 3;
 
 // Parts of an item, on average, that one warp of the merge adds up; more are shared by four.
 constexpr int kFewParts = 8;
@@ -749,7 +754,7 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
   p->unit_shift = p->merge ? kUnitShift : kWholeShift;
   const int64_t tiles = ceil_div(static_cast<int64_t>(max_nodes) * (heads / cache->kv_heads), p->v.rows);
   // (the kernels multiply the number of units by that of the CTAs)
-  if (batch->batch * cache->kv_heads * tiles * ceil_div(cap, 1 << p->unit_shift) > INT64_MAX / (2 * kMaxParts))
+  if (batch->batch * cache->kv_heads * tiles * (kBeginCost + ceil_div(cap, 1 << p->unit_shift)) > INT64_MAX / (2 * kMaxParts))
     return ncm_fail(NCM_EINVAL, "%s: too many keys", what);
   p->grid = std::min(kMaxParts, ctx->num_sms * resident[index].load());
   p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
@@ -813,6 +818,7 @@ int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv
   a.lse = lse;
   a.part = static_cast<float*>(workspace);
   a.unit_shift = p.unit_shift;
+  a.begin_cost = kBeginCost;
   a.err = ctx->d_err;
   const int64_t most_rows = static_cast<int64_t>(max_nodes) * a.group;
   const int64_t items = static_cast<int64_t>(batch->batch) * cache->kv_heads * ceil_div(most_rows, p.v.rows);

@@ -23,6 +23,7 @@ struct TreeArgs {
   float* lse;
   float* part;  // [2 * grid][ROWS][4 + HD]: m, sum of p, m', -, values
   int unit_shift;  // log2 of a unit's keys
+  int begin_cost;  // what beginning an item takes, in units
   int grid;  // CTAs of the attention kernel
   int* err;
 };
@@ -124,17 +125,19 @@ __device__ __forceinline__ long long quotient(long long x, long long d) {
   if (((x | d) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(d);
   return x / d;
 }
-// How `total` units are dealt out: every CTA has `each` consecutive ones, the first `more` one beyond.
+// The work of a sequence: every item is begin_cost places, then its units.
+__device__ __forceinline__ long long places_of(const TreeArgs& a, const Seq& s, int tiles) {
+  return static_cast<long long>(tiles) * a.pools.kv_heads * (a.begin_cost + units_of(a, s));
+}
+// How `total` places are dealt out: `ctas` CTAs (no more than there are places)
+// have consecutive ones each, as evenly as whole places allow.
 struct Deal {
-  long long each;
-  int more;
-  __device__ __forceinline__ Deal(const TreeArgs& a, long long total)
-      : each(quotient(total, a.grid)), more(static_cast<int>(total - each * a.grid)) {}
-  __device__ __forceinline__ long long first(int cta) const { return cta * each + min(cta, more); }
-  __device__ __forceinline__ int owner(long long unit) const {
-    const long long longer = more * (each + 1);
-    return static_cast<int>(unit < longer ? quotient(unit, each + 1) : more + quotient(unit - longer, each));
-  }
+  long long total;
+  int ctas;
+  __device__ __forceinline__ Deal(const TreeArgs& a, long long places)
+      : total(places), ctas(static_cast<int>(min(static_cast<long long>(a.grid), places))) {}
+  __device__ __forceinline__ long long first(int cta) const { return cta >= ctas ? total : quotient(total * cta, ctas); }
+  __device__ __forceinline__ int owner(long long place) const { return static_cast<int>(quotient((place + 1) * ctas - 1, total)); }
 };
 __device__ __forceinline__ long long warp_sum(long long x) {
 #pragma unroll
@@ -157,39 +160,40 @@ __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >
 
 // The segments of one CTA, in order: runs of consecutive units of one item
 // (sequence, kv head, tile of ROWS rows). Every thread walks the same ones.
+// Beginning an item costs begin_cost places, so that a CTA with many short items gets fewer keys.
 template <int ROWS>
 struct Walk {
   long long at, hi, inside;
   int b;
   Seq s;
-  int units, u0, u1;
+  int units, u0, u1, taken;  // (taken: places of the segment)
   int kvh, row0, live_rows;  // (live_rows: rows of the item from row0 on; may be more than ROWS)
   int ctx, key0, key1;
 
   // Whole warps; block 0 reports sequences that do not fit.
   __device__ __forceinline__ Walk(const TreeArgs& a, int block) {
     const int lane = threadIdx.x & 31;
-    auto units_at = [&](int i, bool report) {
+    auto places_at = [&](int i, bool report) {
       if (i >= a.batch.batch) return 0ll;
       const Seq q = load_seq(a, i, report);
-      return static_cast<long long>(tiles_of<ROWS>(a, q)) * a.pools.kv_heads * units_of(a, q);
+      return places_of(a, q, tiles_of<ROWS>(a, q));
     };
     const bool report = block == 0 && threadIdx.x < 32;
-    const long long mine = units_at(lane, report);  // (of the first 32 sequences, which are mostly all)
+    const long long mine = places_at(lane, report);  // (of the first 32 sequences, which are mostly all)
     long long total = mine;
-    for (int i = lane + 32; i < a.batch.batch; i += 32) total += units_at(i, report);
+    for (int i = lane + 32; i < a.batch.batch; i += 32) total += places_at(i, report);
     total = warp_sum(total);
     const Deal deal(a, total);
     at = deal.first(block);
     hi = deal.first(block + 1);
     inside = 0;
-    u0 = u1 = 0;
+    taken = 0;
     b = a.batch.batch;
     if (at >= hi) return;
-    // the sequence that holds unit `at`
+    // the sequence that holds place `at`
     long long x = at;
     for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
-      const long long u = b0 == 0 ? mine : units_at(b0 + lane, false);
+      const long long u = b0 == 0 ? mine : places_at(b0 + lane, false);
       long long before = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -209,21 +213,26 @@ struct Walk {
     }
   }
   __device__ __forceinline__ bool next(const TreeArgs& a) {
-    at += u1 - u0;
-    inside += u1 - u0;
-    u0 = u1 = 0;
-    while (at < hi && b < a.batch.batch) {
+    for (;;) {
+      at += taken;
+      inside += taken;
+      taken = 0;
+      if (at >= hi || b >= a.batch.batch) return false;
       s = load_seq(a, b, false);
       units = units_of(a, s);
-      const int tiles = tiles_of<ROWS>(a, s);
-      if (inside >= static_cast<long long>(units) * tiles * a.pools.kv_heads) {  // (empty sequences too)
+      const int tiles = tiles_of<ROWS>(a, s), places = a.begin_cost + units;
+      if (inside >= places_of(a, s, tiles)) {  // (empty sequences too)
         ++b;
         inside = 0;
         continue;
       }
-      const int item = static_cast<int>(quotient(inside, units));
-      u0 = static_cast<int>(inside - static_cast<long long>(item) * units);
-      u1 = static_cast<int>(min(static_cast<long long>(units), u0 + (hi - at)));
+      const int item = static_cast<int>(quotient(inside, places));
+      const int p0 = static_cast<int>(inside - static_cast<long long>(item) * places);
+      const int p1 = static_cast<int>(min(static_cast<long long>(places), p0 + (hi - at)));
+      taken = p1 - p0;
+      u0 = max(p0 - a.begin_cost, 0);
+      u1 = max(p1 - a.begin_cost, 0);
+      if (u0 == u1) continue;  // the item's units are the next CTA's
       kvh = item / tiles;
       row0 = (item - kvh * tiles) * ROWS;
       live_rows = s.n * a.group - row0;
@@ -232,7 +241,6 @@ struct Walk {
       key1 = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(u1) << a.unit_shift));
       return true;
     }
-    return false;
   }
   __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == units; }
 };
