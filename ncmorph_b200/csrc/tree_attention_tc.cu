@@ -59,19 +59,15 @@ struct TcShape {
   static constexpr int kLoadGroups = SPLITQ && !kCodes ? 1 : 2;
   static constexpr int kThreads = 32 * (8 + 2 + kLoadGroups * kLoadWarps);
   static constexpr int kRowBytes = HD * (kCodes ? 1 : 2);
-  // Keys of a tile: what a row waits for per tile is the same for 64 keys and for
-  // 128, but 128 of 128-wide heads do not fit beside the rest.
-  static constexpr int kBK = HD == 64 ? 128 : 64;
+  static constexpr int kBK = 64;  // keys of a tile
   static constexpr int kSBufs = 128 / kBK;  // buffers of S
-  // Tiles in bf16; codes: raw tiles in flight in front of them (of both groups of
-  // loaders), in shared memory, or (head_dim 128, where that is full) one a group in registers.
-  static constexpr int kStages = kCodes && HD == 64 ? 2 : 4;
-  static constexpr bool kInRegs = kCodes && HD == 128;
-  static constexpr int kRaw = !kCodes || kInRegs ? 0 : 2;
-  static constexpr int kPBufs = kInRegs ? 1 : kSBufs;  // buffers of P, of 128 rows x kBK keys
+  // Tiles in bf16, and for codes the raw tiles in flight in front of them.
+  static constexpr int kStages = HD == 64 ? (kCodes ? 4 : 8) : (kCodes ? 2 : 4);
+  static constexpr int kRaw = kCodes ? 4 : 0;
+  static constexpr int kPBufs = kCodes && HD == 128 ? 1 : 2;  // buffers of P, of 128 rows x kBK keys (one where shared memory is full)
   static constexpr int kPBytes = 256 * kBK;
   // tiles that a group of loaders has asked for before it waits for the first of them
-  static constexpr int kAhead = kLoadGroups == 1 ? 2 : 1;
+  static constexpr int kAhead = kLoadGroups == 1 ? 4 : 2;
   // (a stage's uses all belong to one group of loaders, and to one of softmax warps
   // where those take every other tile: each waits for its own earlier use)
   static_assert(kStages % 2 == 0, "stages per group");
@@ -85,10 +81,9 @@ struct TcShape {
   static constexpr int kBlock = 128 * kBK;  // bytes of 64 dims of a K or V tile
   static constexpr int kV = kK + kStages * kBlocks * kBlock;
   static constexpr int kRawAt = kV + kStages * kBlocks * kBlock;
-  static constexpr int kScale = kRawAt + kRaw * 2 * kBK * kRowBytes;  // [slot][K, V][kBK] f32
-  static constexpr bool kRawScales = kCodes && !kInRegs;
+  static constexpr int kScale = kRawAt + kRaw * 2 * kBK * kRowBytes;  // [slot][K (times log2(e) scale), V][kBK] f32
   static constexpr int kRawScale = kScale + (kCodes ? kScaleSlots * 2 * kBK * 4 : 0);  // [raw][K, V][kBK] f32
-  static constexpr int kBars = kRawScale + (kRawScales ? kRaw * 2 * kBK * 4 : 0);
+  static constexpr int kBars = kRawScale + kRaw * 2 * kBK * 4;
   static constexpr int kSums = kBars + kBarBytes;  // !SPLITQ: the groups' maxima and sums, [group][128]
   static constexpr int kSmem = kSums + (SPLITQ ? 0 : 2 * 128 * 8);
   static constexpr uint32_t kTmemCols = 512;  // S: 2 x 2 x 64, O: 2 x head_dim
@@ -256,8 +251,65 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
           const bool partly = base + BK > min(w.ctx, w.key1);
           // P's buffer is free once the product that read it last is done
           constexpr uint32_t PB = S::kPBufs;
-          if (j >= PB && !wait(&B.pv_done[g][(j - PB) & 1], ((j - PB) >> 1) & 1u)) break;
+          auto p_free = [&] { return j < PB || wait(&B.pv_done[g][(j - PB) & 1], ((j - PB) >> 1) & 1u); };
           uint8_t* prow = smem + S::kP + (PB * g + j % PB) * S::kPBytes + row * 128;
+          // Most tiles: every key is seen, and no score passes the maximum by more than
+          // the slack. That is not waited for: the maximum stays as it is, and the tile is done
+          // again, by the loop below, where a score turns out to pass it. Then nothing stands
+          // between a score and its exponential, and the next 16 scores are under way meanwhile.
+          auto quick = [&] {
+            const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2), minus_m = f2_pack(-m, -m);
+            unsigned long long sum = f2_pack(0.f, 0.f), sum2 = sum;
+            float worst = kFirstMax;
+            uint32_t raw[2][16];
+            tmem_ld_x16(sbase, raw[0]);
+#pragma unroll
+            for (int h = 0; h < BK / 16; ++h) {
+              tmem_wait_ld();
+              uint32_t(&now)[16] = raw[h & 1];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(now[i]));  // (not used before the wait)
+              if (h + 1 < BK / 16) tmem_ld_x16(sbase + 16 * (h + 1), raw[(h + 1) & 1]);
+              float* sc = reinterpret_cast<float*>(now);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const unsigned long long f = CODES ? reinterpret_cast<const unsigned long long*>(scales)[8 * h + i] : up;
+                f2_unpack(f2_fma(f2_pack(sc[2 * i], sc[2 * i + 1]), f, minus_m), sc[2 * i], sc[2 * i + 1]);
+                worst = fmaxf(worst, fmaxf(sc[2 * i], sc[2 * i + 1]));
+              }
+              if (h == BK / 16 - 1) {
+                if (__any_sync(0xffffffffu, exists && worst > kSlack)) return false;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
+              }
+              if (h == 0 && !p_free()) return true;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint32_t e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int k = 8 * c + 2 * i;
+                  unsigned long long p = f2_pack(ex2(sc[k]), ex2(sc[k + 1]));
+                  if (i & 1)
+                    sum2 = f2_add(sum2, p);
+                  else
+                    sum = f2_add(sum, p);
+                  if constexpr (CODES) p = f2_mul(p, reinterpret_cast<const unsigned long long*>(scales)[BK / 2 + 8 * h + k / 2]);
+                  float p0, p1;
+                  f2_unpack(p, p0, p1);
+                  e[i] = pack_rn_bf16x2(p0, p1);
+                }
+                *reinterpret_cast<uint4*>(prow + (h >> 2) * 16384 + (((2 * (h & 3) + c) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+              }
+            }
+            float s0, s1;
+            f2_unpack(f2_add(sum, sum2), s0, s1);
+            l += s0 + s1;
+            return true;
+          };
+          if (partly || !any || !quick()) {
+          if (!p_free()) break;
           // Scores: raw where they take the scale with the exponent (bf16 cache,
           // positive scale), otherwise in units of log2; -inf where hidden.
           const bool late = !CODES && a.scale_log2 > 0.f;
@@ -280,7 +332,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
               const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2);
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const unsigned long long f = CODES ? f2_mul(reinterpret_cast<const unsigned long long*>(scales)[16 * h + i], up) : up;
+                const unsigned long long f = CODES ? reinterpret_cast<const unsigned long long*>(scales)[16 * h + i] : up;
                 f2_unpack(f2_mul(f2_pack(sc[2 * i], sc[2 * i + 1]), f), sc[2 * i], sc[2 * i + 1]);
               }
             }
@@ -361,6 +413,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
             float s0, s1;
             f2_unpack(sum, s0, s1);
             l += s0 + s1;
+          }
           }
           if (!ok) break;
         } else {
@@ -487,19 +540,32 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       const uint32_t ts = tmem + 128 * g, to = tmem + 256 + g * HD;
       uint32_t js = 0, jo = 0, segment = 0;  // products issued, of each kind
       bool ok = true;
+      auto s_ready = [&](uint32_t n) {
+        return mbar_test_wait(&B.k_full[n % NS], (n / NS) & 1u) && (js < 2 || mbar_test_wait(&B.s_free[g][js & 1], ((js - 2) >> 1) & 1u));
+      };
       auto issue_s = [&](uint32_t n) {
         const uint32_t st = n % NS, buf = js & 1u;
-        if (!(ok = tc_wait(&B.k_full[st], (n / NS) & 1u, abort_flag))) return;
-        if (js >= S::kSBufs && !(ok = tc_wait(&B.s_free[g][(js - S::kSBufs) & 1], ((js - S::kSBufs) >> 1) & 1u, abort_flag))) return;
         tc_fence_after();
         const uint64_t db = dk + st * NB * (S::kBlock / 16);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          tc_mma_f16(ts + (js % S::kSBufs) * BK, dq + (k >> 2) * 1024 + 2 * (k & 3), db + (k >> 2) * (S::kBlock / 16) + 2 * (k & 3), id_s,
-                     k != 0 ? 1u : 0u);
+          tc_mma_f16(ts + buf * BK, dq + (k >> 2) * 1024 + 2 * (k & 3), db + (k >> 2) * (S::kBlock / 16) + 2 * (k & 3), id_s, k != 0 ? 1u : 0u);
         tc_commit(&B.s_full[g][buf]);
         tc_commit(&B.k_empty[st]);
         ++js;
+      };
+      auto pv_ready = [&](uint32_t n) {
+        return mbar_test_wait(&B.p_full[g][jo & 1], (jo >> 1) & 1u) && mbar_test_wait(&B.v_full[n % NS], (n / NS) & 1u);
+      };
+      auto issue_pv = [&](uint32_t n, bool first) {
+        const uint32_t st = n % NS, buf = jo & 1u;
+        tc_fence_after();
+        const uint64_t da = dp + (jo % S::kPBufs) * (S::kPBytes / 16), db = dv + st * NB * (S::kBlock / 16);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) tc_mma_f16(to, da + 2 * k, db + k * 128, id_o, !first || k != 0 ? 1u : 0u);
+        tc_commit(&B.pv_done[g][buf]);
+        tc_commit(&B.v_empty[st]);
+        ++jo;
       };
       for (; ok && w.next(a); ++segment) {
         const uint32_t ntiles = (w.key1 - w.key0 + BK - 1) / BK, n0 = number;
@@ -513,20 +579,28 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
           }
           continue;
         }
+        // Whichever product can go next goes: the scores of a tile run ahead of the values'
+        // products by up to two tiles, and neither waits for the other's operands.
         const uint32_t first = n0 + (SPLITQ ? 0 : g);
-        if (first < number) issue_s(first);
-        for (uint32_t n = first; ok && n < number; n += STEP) {
-          // S of the next tile first: it is computed while this one's exponentials run
-          if (n + STEP < number) issue_s(n + STEP);
-          const uint32_t st = n % NS, buf = jo & 1u;
-          if (!ok || !(ok = tc_wait(&B.v_full[st], (n / NS) & 1u, abort_flag) && tc_wait(&B.p_full[g][buf], (jo >> 1) & 1u, abort_flag))) break;
-          tc_fence_after();
-          const uint64_t da = dp + (jo % S::kPBufs) * (S::kPBytes / 16), db = dv + st * NB * (S::kBlock / 16);
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k) tc_mma_f16(to, da + (k >> 2) * 1024 + 2 * (k & 3), db + k * 128, id_o, n != first || k != 0 ? 1u : 0u);
-          tc_commit(&B.pv_done[g][buf]);
-          tc_commit(&B.v_empty[st]);
-          ++jo;
+        uint32_t ns = first, no = first;
+        uint64_t since = 0;
+        uint32_t tries = 0;
+        while (ok && no < number) {
+          if (ns < number && s_ready(ns)) {
+            issue_s(ns);
+            ns += STEP;
+          } else if (no < ns && pv_ready(no)) {
+            issue_pv(no, no == first);
+            no += STEP;
+          } else {  // (bounded, as every wait here)
+            if ((++tries & 63u) == 0u) {
+              const uint64_t now = globaltimer_ns();
+              if (since == 0) since = now;
+              ok = !*abort_flag && now - since <= kWaitLimitNs;
+            }
+            continue;
+          }
+          since = 0;
         }
       }
       if (!ok) fail();
@@ -541,86 +615,72 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
     constexpr int PER = BK * CPR / kLoadThreads;  // 16-byte pieces of a thread, of K and of V: each KPX keys on
     constexpr int KPX = kLoadThreads / CPR;
     static_assert(KPX % 8 == 0, "a thread's pieces have one swizzle");
-    // (rolled where the pieces need no registers of their own: the roles' code shares the instruction cache)
-    constexpr int ROLL = S::kInRegs ? PER : 1;
     const int page_mask = (1 << a.pools.page_shift) - 1;
     const int my_key = tid / CPR, my_c = tid % CPR;
-    uint32_t issued = 0, done = 0;  // of this group's tiles: the numbers group, group + 2, ...
-    uint32_t nodes = 0;             // bit i: the tile issued i tiles ago holds new tokens
-    float scale_of_tile = 0.f;
-    uint4 held[S::kInRegs ? 2 * PER : 1];  // (kInRegs: the tile under way)
+    // A tile is asked for and handed over as one, or, where its places are few (128-wide bf16),
+    // in parts: the keys' places are free long before the values'. us of one and two parts,
+    // 128 rows of eight sequences: 86.7 and 81.4 at head_dim 128, 52.2 and 55.4 at 64.
+    constexpr uint32_t PARTS = !CODES && HD == 128 ? 2 : 1, AHEAD = PARTS * S::kAhead;
+    uint32_t issued = 0, done = 0;  // parts of this group's tiles: the numbers group, group + 2, ...
+    uint32_t nodes = 0;             // bit i: the part issued i parts ago is of new tokens' values
     bool ok = true;
-    // The page of a key of the segment, or -1 behind its last one; reports a page that is not there.
-    auto page_of = [&](int key) {
-      if (key >= w.key1) return -1;
-      const int p = __ldg(a.batch.page_table + w.b * a.batch.table_stride + (key >> a.pools.page_shift));
-      if (p >= 0 && p < a.pools.num_pages) return p;
-      atomicOr(a.err, kErrBadIndex);
-      return -1;
+    // Pages of keys base + lane and base + 32 + lane of the next tile, asked for one tile
+    // ahead of their use, and the places of those keys of this one (-1 behind the segment's
+    // last key, or where the page is not there, which is reported).
+    int page_lo = -1, page_hi = -1, lo = -1, hi = -1;
+    auto ask_pages = [&](int base) {
+      const int32_t* table = a.batch.page_table + w.b * a.batch.table_stride;
+      page_lo = base + lane < w.key1 ? __ldg(table + ((base + lane) >> a.pools.page_shift)) : -1;
+      page_hi = base + 32 + lane < w.key1 ? __ldg(table + ((base + 32 + lane) >> a.pools.page_shift)) : -1;
     };
-    // asks for tile n of the segment, the one at `base`
-    auto issue = [&](uint32_t n, int base) {
-      const uint32_t at = CODES ? smem_u32(smem + S::kRawAt) + (n % (CODES && !S::kInRegs ? S::kRaw : 1)) * 2 * BK * RB + tid * 16
+    auto place_of = [&](int key, int page) {
+      if (key >= w.key1) return -1;
+      if (page < 0 || page >= a.pools.num_pages) {
+        atomicOr(a.err, kErrBadIndex);
+        return -1;
+      }
+      return static_cast<int>(kv_slot(a.pools, page, w.kvh, key & page_mask));
+    };
+    auto begin_tile = [&](int base, int next) {
+      lo = place_of(base + lane, page_lo);
+      hi = place_of(base + 32 + lane, page_hi);
+      if (next < w.key1) ask_pages(next);
+    };
+    // asks for a part of tile n of the segment, the one at `base`
+    auto issue = [&](uint32_t n, int base, uint32_t part) {
+      const uint32_t at = CODES ? smem_u32(smem + S::kRawAt) + (n % (S::kRaw + !S::kRaw)) * 2 * BK * RB + tid * 16
                                 : smem_u32(smem + S::kK) + ((n % NS) * NB + (my_c >> 3)) * S::kBlock + my_key * 128 + (((my_c & 7) ^ (my_key & 7)) << 4);
       constexpr uint32_t TO_X = CODES ? kLoadThreads * 16 : KPX * 128, TO_V = CODES ? BK * RB : S::kV - S::kK;
-      auto fetch = [&](int x, long long byte, bool live) {
-        const uint8_t* k = static_cast<const uint8_t*>(a.pools.k) + byte;
-        const uint8_t* v = static_cast<const uint8_t*>(a.pools.v) + byte;
-        if constexpr (S::kInRegs) {
-          held[2 * x] = live ? __ldg(reinterpret_cast<const uint4*>(k)) : make_uint4(0u, 0u, 0u, 0u);
-          held[2 * x + 1] = live ? __ldg(reinterpret_cast<const uint4*>(v)) : make_uint4(0u, 0u, 0u, 0u);
-        } else {
-          cp16(at + x * TO_X, k, live);
-          cp16(at + TO_V + x * TO_X, v, live);
-        }
-      };
-      if ((1 << a.pools.page_shift) >= BK) {  // the tile is one run of its page
-        const int page = page_of(base);
-        const long long first = page >= 0 ? kv_slot(a.pools, page, w.kvh, base & page_mask) : 0;
-        const int live = page >= 0 ? w.key1 - base : 0;
-#pragma unroll ROLL
-        for (int x = 0; x < PER; ++x) {
-          const bool here = my_key + x * KPX < live;
-          fetch(x, here ? first * RB + tid * 16 + x * (kLoadThreads * 16) : 0, here);
-        }
-      } else {
-#pragma unroll ROLL
-        for (int x = 0; x < PER; ++x) {
-          const int page = page_of(base + my_key + x * KPX);
-          const long long slot = page >= 0 ? kv_slot(a.pools, page, w.kvh, (base + my_key + x * KPX) & page_mask) : 0;
-          fetch(x, page >= 0 ? slot * RB + my_c * 16 : 0, page >= 0);
-        }
-      }
-      if constexpr (CODES) {  // and scales: of key tid % BK, K's and V's by turns of BK threads
+      const uint8_t* k = static_cast<const uint8_t*>(a.pools.k) + my_c * 16;
+      const uint8_t* v = static_cast<const uint8_t*>(a.pools.v) + my_c * 16;
 #pragma unroll
-        for (int x = 0; x < 2 * BK / kLoadThreads; ++x) {
-          const int i = x * kLoadThreads + tid, key = base + (i & (BK - 1)), page = page_of(key);
-          const float* from = (i < BK ? a.pools.k_scale : a.pools.v_scale) + (page >= 0 ? kv_slot(a.pools, page, w.kvh, key & page_mask) : 0);
-          if constexpr (S::kRawScales)
-            cp4(smem_u32(smem + S::kRawScale) + ((n % S::kRaw) * 2 * BK + i) * 4, from, page >= 0);
-          else
-            scale_of_tile = page >= 0 ? *from : 0.f;
-        }
+      for (int x = 0; x < PER; ++x) {  // (KPX divides 32: a piece's keys are all among the first 32, or all behind them)
+        const int place = __shfl_sync(0xffffffffu, x * KPX < 32 ? lo : hi, (my_key + x * KPX) & 31);
+        const long long byte = static_cast<long long>(max(place, 0)) * RB;
+        if (PARTS == 1 || part == 0) cp16(at + x * TO_X, k + byte, place >= 0);
+        if (PARTS == 1 || part == 1) cp16(at + TO_V + x * TO_X, v + byte, place >= 0);
+      }
+      if constexpr (CODES) {  // and scales: of key tid % 64, K's by the first 64 threads, V's by the others
+        static_assert(2 * BK == kLoadThreads && BK == 64, "a scale a thread");
+        const int place = (tid & 32) == 0 ? lo : hi;
+        cp4(smem_u32(smem + S::kRawScale) + ((n % (S::kRaw + !S::kRaw)) * 2 * BK + tid) * 4,
+            (tid < BK ? a.pools.k_scale : a.pools.v_scale) + max(place, 0), place >= 0);
       }
       cp_commit();
-      nodes = nodes << 1 | (base + BK > w.ctx ? 1u : 0u);
+      nodes = nodes << 1 | (part == PARTS - 1 && base + BK > w.ctx ? 1u : 0u);
       ++issued;
     };
-    // waits for the oldest tile under way and hands it to the products
+    // waits for the oldest part under way and hands it to the products
     auto finish = [&] {
-      const uint32_t n = LG * done + group;
+      const uint32_t n = LG * (done / PARTS) + group;
       const int st = n % NS;
-      if (issued - done == S::kAhead)
-        cp_wait<S::kAhead - 1>();
+      if (issued - done == AHEAD)
+        cp_wait<AHEAD - 1>();
       else
         cp_wait<0>();
       if constexpr (CODES) {
-#pragma unroll
-        for (int x = 0; x < 2 * BK / kLoadThreads; ++x) {
-          const int i = x * kLoadThreads + tid;
-          reinterpret_cast<float*>(smem + S::kScale)[(n % S::kScaleSlots) * 2 * BK + i] =
-              S::kRawScales ? reinterpret_cast<const float*>(smem + S::kRawScale)[(n % (S::kRaw + !S::kRaw)) * 2 * BK + i] : scale_of_tile;
-        }
+        const float scale = reinterpret_cast<const float*>(smem + S::kRawScale)[(n % (S::kRaw + !S::kRaw)) * 2 * BK + tid];
+        reinterpret_cast<float*>(smem + S::kScale)[(n % S::kScaleSlots) * 2 * BK + tid] = tid < BK ? scale * a.scale_log2 : scale;
         const uint32_t from = smem_u32(smem + S::kRawAt) + (n % (S::kRaw + !S::kRaw)) * 2 * BK * RB + tid * 16;
         const uint32_t to = smem_u32(smem + S::kK) + (st * NB + (my_c >> 2)) * S::kBlock + my_key * 128;
         // (128-wide rows: half of the lanes store their second eight values first, so that a
@@ -630,13 +690,12 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (n >= NS && !warp_wait(kv ? &B.v_empty[st] : &B.k_empty[st], ((n / NS) - 1) & 1u)) return false;
+          uint4 raw[PER];
+#pragma unroll
+          for (int x = 0; x < PER; ++x) raw[x] = lds128(from + kv * BK * RB + x * kLoadThreads * 16);
 #pragma unroll
           for (int x = 0; x < PER; ++x) {
-            uint4 v;
-            if constexpr (S::kInRegs)
-              v = held[2 * x + kv];
-            else
-              v = lds128(from + kv * BK * RB + x * kLoadThreads * 16);
+            const uint4 v = raw[x];
             const uint32_t e[4] = {flip ? v.z : v.x, flip ? v.w : v.y, flip ? v.x : v.z, flip ? v.y : v.w};
             uint32_t o[8];
 #pragma unroll
@@ -674,8 +733,8 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&B.k_full[st]);
-          mbar_arrive(&B.v_full[st]);
+          if (PARTS == 1 || done % PARTS == 0) mbar_arrive(&B.k_full[st]);
+          if (PARTS == 1 || done % PARTS == 1) mbar_arrive(&B.v_full[st]);
         }
       }
       ++done;
@@ -685,24 +744,33 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       const int ntiles = (w.key1 - w.key0 + BK - 1) / BK;
       const uint32_t first = number;
       number += ntiles;
-      for (int t = (group - first) & (LG - 1); ok && t < ntiles; t += LG) {
+      const int t0 = (group - first) & (LG - 1);
+      ask_pages(w.key0 + t0 * BK);
+      for (int t = t0; ok && t < ntiles; t += LG) {
         const uint32_t n = first + t;
-        if (issued - done == S::kAhead) ok = finish();
-        if constexpr (!CODES) {
-          // The stage's last tile must be done with. Where it is not yet, the tiles under way
-          // are handed over first: the products may be waiting for just those.
-          if (ok && n >= NS) {
-            const uint32_t parity = ((n / NS) - 1) & 1u;
-            auto free_now = [&] {
-              int f = 1;
-              if (lane == 0) f = mbar_test_wait(&B.k_empty[n % NS], parity) && mbar_test_wait(&B.v_empty[n % NS], parity);
-              return __shfl_sync(0xffffffffu, f, 0) != 0;
-            };
-            while (ok && done < issued && !free_now()) ok = finish();
-            ok = ok && warp_wait(&B.k_empty[n % NS], parity) && warp_wait(&B.v_empty[n % NS], parity);
+        begin_tile(w.key0 + t * BK, w.key0 + (t + LG) * BK);
+#pragma unroll 1
+        for (uint32_t part = 0; ok && part < PARTS; ++part) {
+          if (issued - done == AHEAD) ok = finish();
+          if constexpr (!CODES) {
+            // The place's last tile must be done with. Where it is not yet, the parts under way
+            // are handed over first: the products may be waiting for just those.
+            if (ok && n >= NS) {
+              // (a tile's values are done with after its keys)
+              uint64_t* bar = PARTS == 2 && part == 0 ? &B.k_empty[n % NS] : &B.v_empty[n % NS];
+              const uint32_t parity = ((n / NS) - 1) & 1u;
+              auto free_now = [&] {
+                int f = 1;
+                if (lane == 0) f = mbar_test_wait(bar, parity);
+                return __shfl_sync(0xffffffffu, f, 0) != 0;
+              };
+              while (ok && done < issued && !free_now()) ok = finish();
+              ok = ok && warp_wait(bar, parity);
+              if (PARTS == 1) ok = ok && warp_wait(&B.k_empty[n % NS], parity);
+            }
           }
+          if (ok) issue(n, w.key0 + t * BK, part);
         }
-        if (ok) issue(n, w.key0 + t * BK);
       }
     }
     while (ok && done < issued) ok = finish();
