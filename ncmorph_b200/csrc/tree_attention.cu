@@ -676,24 +676,21 @@ constexpr Variant variant() {
   return Variant{tree_attention_kernel<HD, FMT, NT, RG, KG>, S::kRows, S::kThreads, S::kSmem};
 }
 
-// By the rows of one kv head: 8, 16, 32 or 64 rows a tile. Few rows take the
+// By the rows of one kv head: 8, 16 or 32 rows a tile. Few rows take the
 // keys four groups at a time, more share each tile among row groups.
-constexpr int kSizes = 4;
+constexpr int kSizes = 3;
 template <int FMT>
 struct Variants {
-  static constexpr Variant hd64[kSizes] = {variant<64, FMT, 1, 1, 4>(), variant<64, FMT, 2, 1, 4>(), variant<64, FMT, 4, 1, 4>(),
-                                           variant<64, FMT, 4, 2, 2>()};
-  static constexpr Variant hd128[kSizes] = {variant<128, FMT, 1, 1, 4>(), variant<128, FMT, 2, 1, 4>(), variant<128, FMT, 2, 2, 2>(),
-                                            variant<128, FMT, 2, 4, 1>()};
+  static constexpr Variant hd64[kSizes] = {variant<64, FMT, 1, 1, 4>(), variant<64, FMT, 2, 1, 4>(), variant<64, FMT, 4, 1, 4>()};
+  static constexpr Variant hd128[kSizes] = {variant<128, FMT, 1, 1, 4>(), variant<128, FMT, 2, 1, 4>(), variant<128, FMT, 2, 2, 2>()};
 };
 
 // Rows of one kv head that stay with the mma.sync kernel. More go to the tcgen05
 // kernel, whose tiles have 128 rows. us of both, mma.sync / tcgen05 (eight
-// sequences of 1 to 16 thousand tokens, 8 kv heads): 64 rows, bf16: 56 / 79 at
-// head_dim 64, 81 / 107 at 128, int8: 66 / 77 and 92 / 111; 128 rows, bf16: 100 /
-// 89 and 160 / 125, int8: 113 / 92 and 177 / 126; 256 rows: 187 / 131, 300 / 227, 207 /
-// 148 and 326 / 219.
-constexpr int64_t kFewRows = 64;
+// sequences of 1 to 16 thousand tokens, 8 kv heads): 32 rows, bf16: 29 / 40 at
+// head_dim 64, 44 / 63 at 128, int8: 34 / 44 and 48 / 65; 48 rows: 40 / 41, 67 / 64,
+// 48 / 45 and 78 / 69; 64 rows: 41 / 42, 68 / 65, 49 / 45 and 79 / 70.
+constexpr int64_t kFewRows = 32;
 Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
   const bool wide = c->head_dim == 128;
   if (rows > kFewRows) {
@@ -703,7 +700,7 @@ Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
   const Variant* v = c->format == NCM_KV_BF16   ? (wide ? Variants<NCM_KV_BF16>::hd128 : Variants<NCM_KV_BF16>::hd64)
                      : c->format == NCM_KV_INT8 ? (wide ? Variants<NCM_KV_INT8>::hd128 : Variants<NCM_KV_INT8>::hd64)
                                                 : (wide ? Variants<NCM_KV_E4M3>::hd128 : Variants<NCM_KV_E4M3>::hd64);
-  const int i = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
+  const int i = rows <= 8 ? 0 : rows <= 16 ? 1 : 2;
   *index = (c->format * 2 + wide) * kSizes + i;
   return v[i];
 }

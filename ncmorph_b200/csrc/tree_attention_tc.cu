@@ -54,9 +54,10 @@ struct TcShape {
   static constexpr int kQTiles = SPLITQ ? 2 : 1;
   static constexpr int kRows = 128 * kQTiles;
   // Two groups of loaders take every other tile, so that one's waits and conversion run
-  // beside the other's. A bf16 tile that 256 rows share lasts long enough for one
-  // group, which leaves 128 registers a thread.
-  static constexpr int kLoadGroups = SPLITQ && !kCodes ? 1 : 2;
+  // beside the other's. A tile that 256 rows share lasts long enough for one group, which
+  // leaves 128 registers a thread (int8, eight sequences of 64 tokens: 80.3 us with two
+  // groups, 77.5 with one; 128 rows, bf16: 45.5 and 51.9).
+  static constexpr int kLoadGroups = SPLITQ ? 1 : 2;
   static constexpr int kThreads = 32 * (8 + 2 + kLoadGroups * kLoadWarps);
   static constexpr int kRowBytes = HD * (kCodes ? 1 : 2);
   static constexpr int kBK = 64;  // keys of a tile
@@ -190,11 +191,9 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
     *abort_flag = 1;
     atomicOr(a.err, kErrWaitTimeout);
   };
-  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {  // one lane waits for its warp
-    int done = 1;
-    if (lane == 0) done = tc_wait(bar, parity, abort_flag);
-    return __shfl_sync(0xffffffffu, done, 0) != 0;
-  };
+  // (every lane asks: one that asks for its warp and tells the others takes a tenth of the
+  // kernel's time more)
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag)) != 0; };
   Walk<ROWS> w(a, blockIdx.x);
   uint32_t number = 0;  // of the segment's first tile: they are numbered over all segments
 
@@ -249,9 +248,10 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
           const float4* scales = reinterpret_cast<const float4*>(smem + S::kScale + ((n0 + t) % S::kScaleSlots) * 2 * BK * 4);
           const int base = w.key0 + t * BK;
           const bool partly = base + BK > min(w.ctx, w.key1);
-          // P's buffer is free once the product that read it last is done
+          // P's buffer is free once the product that read it last is done. With two buffers that is
+          // so already: the scores' product was issued behind it, and so is done after it.
           constexpr uint32_t PB = S::kPBufs;
-          auto p_free = [&] { return j < PB || wait(&B.pv_done[g][(j - PB) & 1], ((j - PB) >> 1) & 1u); };
+          auto p_free = [&] { return PB == 2 || j < PB || wait(&B.pv_done[g][(j - PB) & 1], ((j - PB) >> 1) & 1u); };
           uint8_t* prow = smem + S::kP + (PB * g + j % PB) * S::kPBytes + row * 128;
           // Most tiles: every key is seen, and no score passes the maximum by more than
           // the slack. That is not waited for: the maximum stays as it is, and the tile is done
@@ -579,14 +579,14 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
           }
           continue;
         }
-        // Whichever product can go next goes: the scores of a tile run ahead of the values'
-        // products by up to two tiles, and neither waits for the other's operands.
+        // Whichever product can go next goes: the scores run ahead of the values' products
+        // by up to two tiles, and neither waits for the other's operands.
         const uint32_t first = n0 + (SPLITQ ? 0 : g);
         uint32_t ns = first, no = first;
         uint64_t since = 0;
         uint32_t tries = 0;
         while (ok && no < number) {
-          if (ns < number && s_ready(ns)) {
+          if (ns < number && js < jo + 2 && s_ready(ns)) {
             issue_s(ns);
             ns += STEP;
           } else if (no < ns && pv_ready(no)) {
@@ -759,11 +759,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
               // (a tile's values are done with after its keys)
               uint64_t* bar = PARTS == 2 && part == 0 ? &B.k_empty[n % NS] : &B.v_empty[n % NS];
               const uint32_t parity = ((n / NS) - 1) & 1u;
-              auto free_now = [&] {
-                int f = 1;
-                if (lane == 0) f = mbar_test_wait(bar, parity);
-                return __shfl_sync(0xffffffffu, f, 0) != 0;
-              };
+              auto free_now = [&] { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)) != 0; };
               while (ok && done < issued && !free_now()) ok = finish();
               ok = ok && warp_wait(bar, parity);
               if (PARTS == 1) ok = ok && warp_wait(&B.k_empty[n % NS], parity);
