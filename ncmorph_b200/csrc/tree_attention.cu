@@ -545,8 +545,8 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
 
 // Adds up the partial sums of a row of an item (blockIdx.x: sequence and kv
 // head, blockIdx.y: 4 / WPR rows of the sequence's rows), in an order that the
-// split alone decides. WPR warps share a row: all four of the block where an item
-// of few long sequences has tens of parts, one where it has a few. What the caller
+// split alone decides. WPR warps share a row: all four of the block where there are few
+// rows (kManyRows), otherwise one. What the caller
 // gave is read before the wait: the attention kernel does not let this one start
 // ahead of its own end, and the kernels in front of both are done by then.
 constexpr int kMaxParts = 2048;  // CTAs of the attention kernel at most
@@ -714,8 +714,10 @@ constexpr int kUnitShift = 7;
 // (tcgen05), e4m3, head_dim 128: 73, 58.0, 55.8, 55.9; one long sequence: no difference.
 constexpr int kBeginCost = 3;
 
-// Parts of an item, on average, that one warp of the merge adds up; more are shared by four.
-constexpr int kFewParts = 8;
+// Rows of the merge an SM, from which one warp adds up a row; fewer are shared by four
+// warps each. us of four / one: 256 rows of 9 parts: 19.9 / 20.6, 512 rows of 55:
+// 45.1 / 45.3 (head_dim 128: 34.4 / 35.3), 2048 rows of 18: 76.2 / 72.9, 4096 of 9: 146 / 139.
+constexpr int kManyRows = 6;
 
 struct Plan {
   Variant v;
@@ -827,10 +829,10 @@ int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv
   }
   if (p.merge) {
     Launch _launch(ctx, KID_ATTENTION, st);
-    const bool wide = cache->head_dim == 128, few = kFewParts * items >= p.grid;
-    auto merge = few ? (wide ? tree_merge_kernel<128, 1> : tree_merge_kernel<64, 1>)
-                     : (wide ? tree_merge_kernel<128, 4> : tree_merge_kernel<64, 4>);
-    NCM_CUDA_TRY(launch_pdl(merge, dim3(batch->batch * cache->kv_heads, ceil_div(most_rows, few ? 4 : 1)), dim3(128), 0, st, 1, a, p.v.rows));
+    const bool wide = cache->head_dim == 128, few = static_cast<int64_t>(batch->batch) * cache->kv_heads * most_rows < kManyRows * ctx->num_sms;
+    auto merge = few ? (wide ? tree_merge_kernel<128, 4> : tree_merge_kernel<64, 4>)
+                     : (wide ? tree_merge_kernel<128, 1> : tree_merge_kernel<64, 1>);
+    NCM_CUDA_TRY(launch_pdl(merge, dim3(batch->batch * cache->kv_heads, ceil_div(most_rows, few ? 1 : 4)), dim3(128), 0, st, 1, a, p.v.rows));
   }
   return NCM_OK;
 }
