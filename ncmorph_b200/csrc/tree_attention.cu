@@ -28,6 +28,12 @@
 // A maximum is only moved when a score passes it by 2^8, so most tiles
 // neither reduce over lanes nor rescale.
 //
+// Bound: the cache's bytes with few rows (single tokens of 32 sequences of up to
+// 32768 tokens, 32 query over 8 kv heads of 64, int8: 70 us, 5.6 TB/s, 0.85 of a
+// copy), the issue slots of softmax and conversion with 32 rows (eight tokens of eight
+// sequences, int8: 34 us, 1.6 TB/s). A short context (4 sequences of 200 tokens) takes
+// 5.7 us: one launch, and a chain of four loads.
+//
 // Split: items are cut into units of unit_keys keys, and every CTA of one wave
 // takes the same number of consecutive units, whatever the sequences' lengths
 // are (they are known on the device only). A CTA that ends inside an item

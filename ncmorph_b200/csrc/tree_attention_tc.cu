@@ -3,22 +3,26 @@
 // 128-row tensor-core tile (rows: nodes x the query heads of one kv head). Per key
 // tile of 64:
 //   S = Q K^T    tcgen05.mma M=128 N=64 K=head_dim, f32 in tensor memory (two buffers)
-//   softmax      one thread per row; P (bf16) into a 128-byte-swizzled tile (two buffers)
+//   softmax      one thread per row; P (bf16) into a 128-byte-swizzled tile
 //   O += P V     tcgen05.mma M=128 N=head_dim K=64, accumulated in tensor memory
-// Two groups of four softmax warps work side by side, because one row's tile is
-// a chain of waits (scores, maximum, exponentials, hand-over) three times as long as
-// its exponentials: with up to 128 rows they take every other key tile and add
-// their sums up at the end, with more (head_dim 64) each has 128 rows of its own.
-// Two more warps issue the groups' products; eight load. Every key
+// Two groups of four softmax warps work side by side: with up to 128 rows they
+// take every other key tile and add their sums up at the end, with more
+// (head_dim 64) each has 128 rows of its own. One warp per group issues its
+// products, in whatever order their operands come; the others load. Every key
 // and value is fetched and, for int8 and e4m3, turned into bf16 (exactly) once per CTA,
 // whatever the number of rows; in the mma.sync kernel each 8 to 32 rows do that again.
 // A key's scale multiplies its scores, a value's scale its probability. V is
 // taken as it lies in the cache, head_dim contiguous: the second product's B
 // operand is MN-major.
 //
-// Bound: with more than about 64 rows the exponentials (16 a clock and SM: 128
-// rows of 64 keys take 512 clocks, the two products 256 at head_dim 64), with fewer
-// the cache's bytes. The maximum moves only past 2^8 (kSlack), as in the other
+// Bound: the exponentials (16 a clock and SM: 64 keys of 128 rows take 512 clocks, the
+// two products 256 at head_dim 64 and 512 at 128). Two trees of 64 tokens over up to 131072
+// tokens, bf16, head_dim 64 (256 rows): 139 us, 525 TFLOP/s; the special-function unit
+// is busy 51 % of the kernel's time, and a group's 64 keys take 2000 clocks, 1024 of
+// them exponentials of both groups. Trees of 26 tokens of eight sequences of up to 8191 tokens, e4m3,
+// head_dim 128 (104 rows): 48 us, 179 TFLOP/s; a CTA has about ten tiles of each group there,
+// and its start (a chain of lookups and the first keys: 10000 clocks), the sums' way out and
+// the merge are half of the time. The maximum moves only past 2^8 (kSlack), as in the other
 // kernel; then O is rescaled in tensor memory.
 //
 // A value row of a new token that holds a NaN or an infinity and is hidden from some rows
@@ -61,11 +65,11 @@ struct TcShape {
   static constexpr int kThreads = 32 * (8 + 2 + kLoadGroups * kLoadWarps);
   static constexpr int kRowBytes = HD * (kCodes ? 1 : 2);
   static constexpr int kBK = 64;  // keys of a tile
-  static constexpr int kSBufs = 128 / kBK;  // buffers of S
   // Tiles in bf16, and for codes the raw tiles in flight in front of them.
   static constexpr int kStages = HD == 64 ? (kCodes ? 4 : 8) : (kCodes ? 2 : 4);
   static constexpr int kRaw = kCodes ? 4 : 0;
-  static constexpr int kPBufs = kCodes && HD == 128 ? 1 : 2;  // buffers of P, of 128 rows x kBK keys (one where shared memory is full)
+  // Buffers of P, of 128 rows x kBK keys (one where shared memory is full).
+  static constexpr int kPBufs = kCodes && HD == 128 ? 1 : 2;
   static constexpr int kPBytes = 256 * kBK;
   // tiles that a group of loaders has asked for before it waits for the first of them
   static constexpr int kAhead = kLoadGroups == 1 ? 4 : 2;
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         if (!wait(&B.s_full[g][buf], (j >> 1) & 1u)) break;
         if (busy) {
           tc_fence_after();
-          const uint32_t sbase = tmem + lanes + 128 * g + (j % S::kSBufs) * BK;
+          const uint32_t sbase = tmem + lanes + 128 * g + (j & 1u) * BK;
           const float4* scales = reinterpret_cast<const float4*>(smem + S::kScale + ((n0 + t) % S::kScaleSlots) * 2 * BK * 4);
           const int base = w.key0 + t * BK;
           const bool partly = base + BK > min(w.ctx, w.key1);
