@@ -135,7 +135,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     the softmax sums [T, heads] f32. A new token sees every key in front of the new
     tokens, itself and the earlier new ones; with tree_mask [T, words] int32 those
     new tokens j whose bit j % 32 of word j / 32 is set. max_nodes bounds the new tokens of
-    a sequence. scale defaults to head_dim ** -0.5. A token that sees nothing gets
+    a sequence (at most 1024; a sequence with more is skipped and reported by
+    device.sync). scale defaults to head_dim ** -0.5. A token that sees nothing gets
     zeros and -inf."""
     dev, hd = cache.device, cache.head_dim
     if heads is None:
@@ -148,8 +149,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     b = _batch(cache, token_start, kv_lens, page_table, T)
     words = 0
     if tree_mask is not None:
-        if not isinstance(tree_mask, torch.Tensor) or tree_mask.dim() != 2 or tree_mask.dtype != i32 or tree_mask.device != dev or tree_mask.shape[0] != T or \
-                not tree_mask.is_contiguous():
+        if not isinstance(tree_mask, torch.Tensor) or tree_mask.dim() != 2 or tree_mask.dtype != i32 or \
+                tree_mask.device != dev or tree_mask.shape[0] != T or not tree_mask.is_contiguous():
             raise ValueError(f"tree_mask must be a contiguous int32 [{T}, words] tensor on {dev}")
         words = tree_mask.shape[1]
     if out is None:

@@ -325,6 +325,8 @@ def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, tok
         r.num_tokens = tokens.shape[0]
         r.token_start = need_vec(token_start, i32, "token_start", dev, R + 1)
         r.prompt_lens = need_vec(prompt_lens, i32, "prompt_lens", dev, R)
+        if r.num_tokens == 0:  # (an empty tensor has no address; no history yet is a history)
+            r.tokens = r.token_start
     elif prompt_lens is not None or token_start is not None:
         raise ValueError("token_start and prompt_lens need tokens")
     r.repetition = need_vec(repetition, f32, "repetition", dev, R)

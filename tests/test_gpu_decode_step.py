@@ -1030,3 +1030,17 @@ def test_refusals_of_sizes(cuda_dev):
         with pytest.raises(_lib.NcmError):
             _lib.call("ncm_logits_process", context_of(cache.device), x.data_ptr(), ncm_model.LOGIT_TYPES[torch.float32], 32, x.data_ptr(),
                       ncm_model.LOGIT_TYPES[torch.float32], 32, value if field == "rows" else 1, 32, ctypes.byref(r), raw_stream(cache.device))
+
+
+def test_no_history_yet(cuda_dev):
+    """Empty lists are lists: the first step of a generation has no tokens."""
+    from ncmorph_b200 import ncm_model
+    x = torch.randn((2, 50), device=cuda_dev)
+    i32 = lambda *z: torch.tensor(z, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    ones = torch.full((2,), 1.7, device=cuda_dev)
+    args = dict(tokens=i32(), token_start=i32(0, 0, 0), repetition=ones, frequency=ones, presence=ones, prompt_lens=i32(0, 0),
+                bias=torch.zeros(0, device=cuda_dev), bias_ids=i32(), bias_start=i32(0, 0, 0))
+    assert torch.equal(ncm_model.process_logits(x, **args), x)
+    args["tokens"], args["token_start"] = i32(), i32(0, 0, 1)  # a bound past the (empty) list
+    assert torch.equal(ncm_model.process_logits(x, **args), x)
+    expect_range_error(cuda_dev)
