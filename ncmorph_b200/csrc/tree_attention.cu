@@ -19,7 +19,8 @@
 // Codes are used as they are: int8 and e4m3 values are exact in f16, a key's
 // scale multiplies its scores, and a value's scale s enters its probability's
 // exponent, p' = 2^(t + log2 s - m'), with a maximum m' of its own. P is then f16,
-// which costs 2^-12 of each term. Q is bf16 and becomes f16 with a power of two
+// which costs 2^-12 of each term, or 2^-32 of the row's largest (lifted by 2^7, the
+// largest is at 2^7 or above, and f16's steps end at 2^-24). Q is bf16 and becomes f16 with a power of two
 // of its row taken out; what is then below f16's range is 2^-30 of the
 // row's largest. A bf16 cache is multiplied in bf16 (its values do not fit f16's
 // range), with P rounded to bf16: 2^-9 of each term, about as much again as the output's
@@ -48,6 +49,7 @@ namespace ncm {
 namespace {
 
 constexpr int kTile = 32;  // keys of one ring stage
+constexpr float kLift = 7.f;  // f16 probabilities are lifted by 2^7; with the slack they stay below 2^15
 
 // c += A B, m16n8k16; HALF: f16 operands, otherwise bf16.
 template <bool HALF>
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
           if constexpr (CODES) {
             topv[nt][e] = fmaxf(fmaxf(sc[0][nt][e] + vlog[0][0], sc[0][nt][2 + e] + vlog[0][1]),
                                 fmaxf(sc[1][nt][e] + vlog[1][0], sc[1][nt][2 + e] + vlog[1][1]));
-            move |= topv[nt][e] > mv[nt][e] + kSlack;
+            move |= topv[nt][e] > mv[nt][e] + (kSlack + kLift);
           }
         }
       if (__any_sync(0xffffffffu, move)) {
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
               x = topv[nt][e];
 #pragma unroll
               for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
-              x = fmaxf(x, mv[nt][e]);
+              x = fmaxf(x - kLift, mv[nt][e]);
               f = ex2(mv[nt][e] - x);
               mv[nt][e] = x;
             }

@@ -506,6 +506,27 @@ def test_sharp_and_wide_scores(cuda_dev, dtype, new, hd):
         check_attention(out, lse, attend_ref(w, q, 4, None, scale))
 
 
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("n,heads", [(1, 1), (4, 8), (20, 4)])
+def test_many_small_terms_beside_a_large_one(cuda_dev, dtype, n, heads):
+    """One key takes nearly all of the weight, with zeros in half of its value's columns;
+    there 4000 keys of weight 2^-26 each are all there is, and not lost."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, dtype, [4000 + n], [n], 1, 64, 16)
+    w.k.zero_()
+    w.v.fill_(1.0)
+    w.k[7, 0] = 1.0
+    w.v[7, 32:] = 0.0
+    w.fill()
+    q = torch.zeros((n, heads * 64), dtype=torch.bfloat16)
+    q[:, ::64] = 18.0  # 18 log2(e) = 25.97
+    out = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=n, scale=1.0)
+    o, _, to, _ = attend_ref(w, q, heads, None, 1.0)
+    # f32 scores of 18 (2^-19), two roundings to 16 bits, and f16 half steps of 2^-32 of the largest term
+    tol = 2.0 ** -18 * o.abs() + 2 * BF * o.abs() + (4000 * 2.0 ** -32 if dtype != torch.bfloat16 else 0)
+    assert torch.all((out.cpu().double() - o).abs() <= tol)
+
+
 def test_many_sequences_and_strided_rows(cuda_dev):
     """More sequences than a warp scans at once, empty ones among them, q and out
     as column slices of wider rows; rows behind the last sequence stay."""
