@@ -196,52 +196,52 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
   if (threadIdx.x < a.tokens) slot_of[0][threadIdx.x] = slot_of_row<APPEND>(a, t0 + threadIdx.x);
   __syncthreads();
   for (int turn = 0; t0 < a.batch.rows; t0 += t_step, turn ^= 1) {
-  const int* slots = slot_of[turn];
-  uint16_t* rows = (is_v ? a.v : a.k) + t0 * stride + h * HD + piece * 8;
-  if (threadIdx.x < a.tokens) slot_of[turn ^ 1][threadIdx.x] = slot_of_row<APPEND>(a, t0 + t_step + threadIdx.x);
-  for (int i0 = 0; i0 < a.tokens; i0 += BATCH * step) {
-    uint4 x[BATCH];
-    float scale[BATCH];
-    long long at[BATCH];
+    const int* slots = slot_of[turn];
+    uint16_t* rows = (is_v ? a.v : a.k) + t0 * stride + h * HD + piece * 8;
+    if (threadIdx.x < a.tokens) slot_of[turn ^ 1][threadIdx.x] = slot_of_row<APPEND>(a, t0 + t_step + threadIdx.x);
+    for (int i0 = 0; i0 < a.tokens; i0 += BATCH * step) {
+      uint4 x[BATCH];
+      float scale[BATCH];
+      long long at[BATCH];
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      const int i = i0 + k * step + first;
-      const int slot = !idle && i < a.tokens ? slots[i] : -1;
-      at[k] = slot < 0 ? -1 : kv_slot(a.pools, slot >> a.pools.page_shift, h, slot & ((1 << a.pools.page_shift) - 1));
-      x[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (at[k] < 0) continue;
-      if constexpr (APPEND) {
-        x[k] = __ldcs(reinterpret_cast<const uint4*>(rows + i * stride));
-      } else if constexpr (CODES) {
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + at[k] * HD);
-        x[k].x = c.x;
-        x[k].y = c.y;
-        scale[k] = scales[at[k]];
-      } else {
-        x[k] = *reinterpret_cast<const uint4*>(codes + at[k] * (HD * EB));
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      uint16_t* row = rows + (i0 + k * step + first) * stride;
-      if constexpr (APPEND && CODES) {
-        const uint32_t top = row_top<LPR>(x[k]);
-        if (at[k] >= 0) {
-          float sc;
-          *reinterpret_cast<uint2*>(codes + at[k] * HD) = quantise8<FMT>(x[k], top, &sc);
-          if (piece == 0) scales[at[k]] = sc;
+      for (int k = 0; k < BATCH; ++k) {
+        const int i = i0 + k * step + first;
+        const int slot = !idle && i < a.tokens ? slots[i] : -1;
+        at[k] = slot < 0 ? -1 : kv_slot(a.pools, slot >> a.pools.page_shift, h, slot & ((1 << a.pools.page_shift) - 1));
+        x[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (at[k] < 0) continue;
+        if constexpr (APPEND) {
+          x[k] = __ldcs(reinterpret_cast<const uint4*>(rows + i * stride));
+        } else if constexpr (CODES) {
+          const uint2 c = *reinterpret_cast<const uint2*>(codes + at[k] * HD);
+          x[k].x = c.x;
+          x[k].y = c.y;
+          scale[k] = scales[at[k]];
+        } else {
+          x[k] = *reinterpret_cast<const uint4*>(codes + at[k] * (HD * EB));
         }
-      } else if (at[k] >= 0) {
-        if constexpr (APPEND)
-          *reinterpret_cast<uint4*>(codes + at[k] * (HD * EB)) = x[k];
-        else if constexpr (CODES)
-          *reinterpret_cast<uint4*>(row) = dequantise8<FMT>(x[k].x, x[k].y, scale[k]);
-        else
-          *reinterpret_cast<uint4*>(row) = x[k];
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        uint16_t* row = rows + (i0 + k * step + first) * stride;
+        if constexpr (APPEND && CODES) {
+          const uint32_t top = row_top<LPR>(x[k]);
+          if (at[k] >= 0) {
+            float sc;
+            *reinterpret_cast<uint2*>(codes + at[k] * HD) = quantise8<FMT>(x[k], top, &sc);
+            if (piece == 0) scales[at[k]] = sc;
+          }
+        } else if (at[k] >= 0) {
+          if constexpr (APPEND)
+            *reinterpret_cast<uint4*>(codes + at[k] * (HD * EB)) = x[k];
+          else if constexpr (CODES)
+            *reinterpret_cast<uint4*>(row) = dequantise8<FMT>(x[k].x, x[k].y, scale[k]);
+          else
+            *reinterpret_cast<uint4*>(row) = x[k];
+        }
       }
     }
-  }
-  __syncthreads();
+    __syncthreads();
   }
 }
 

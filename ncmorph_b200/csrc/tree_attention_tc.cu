@@ -287,7 +287,10 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
               }
-              if (h == 0 && !p_free()) return true;
+              if (h == 0 && !p_free()) {
+                tmem_wait_ld();
+                return true;
+              }
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 uint32_t e[4];
@@ -313,111 +316,110 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
             return true;
           };
           if (partly || !any || !quick()) {
-          if (!p_free()) break;
-          // Scores: raw where they take the scale with the exponent (bf16 cache,
-          // positive scale), otherwise in units of log2; -inf where hidden.
-          const bool late = !CODES && a.scale_log2 > 0.f;
-          const float scale = late ? a.scale_log2 : 1.f;
-          // 32 keys at a time, so that a row's scores fit beside the rest in 96
-          // registers. The loop stays rolled: the roles' code together must not
-          // outgrow the instruction cache.
+            if (!p_free()) break;
+            // Scores: raw where they take the scale with the exponent (bf16 cache,
+            // positive scale), otherwise in units of log2; -inf where hidden.
+            const bool late = !CODES && a.scale_log2 > 0.f;
+            const float scale = late ? a.scale_log2 : 1.f;
+            // 32 keys at a time, in a rolled loop: the roles' code together must not
+            // outgrow the instruction cache.
 #pragma unroll 1
-          for (int h = 0; h < BK / 32; ++h) {
-            uint32_t raw[32];
-            float* sc = reinterpret_cast<float*>(raw);
-            tmem_ld_x32(sbase + 32 * h, raw);
-            tmem_wait_ld();
-            if (h == BK / 32 - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
-            }
-            if (!late) {
-              const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const unsigned long long f = CODES ? reinterpret_cast<const unsigned long long*>(scales)[16 * h + i] : up;
-                f2_unpack(f2_mul(f2_pack(sc[2 * i], sc[2 * i + 1]), f), sc[2 * i], sc[2 * i + 1]);
+            for (int h = 0; h < BK / 32; ++h) {
+              uint32_t raw[32];
+              float* sc = reinterpret_cast<float*>(raw);
+              tmem_ld_x32(sbase + 32 * h, raw);
+              tmem_wait_ld();
+              if (h == BK / 32 - 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
               }
-            }
-            uint32_t seen = 0xFFFFFFFFu;
-            if (partly) {
-              const int k0 = base + 32 * h;
-              seen = !exists ? 0u
-                             : first_bits(w.key1 - k0) & (a.mask == nullptr
-                                                              ? first_bits(w.ctx + node - k0 + 1)
-                                                              : mask_window(a.mask + token * a.mask_words, a.mask_words, k0 - w.ctx));
+              if (!late) {
+                const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((seen >> i) & 1u)) sc[i] = -INFINITY;
-            }
-            float x4[4] = {sc[0], sc[1], sc[2], sc[3]};
-#pragma unroll
-            for (int i = 4; i < 28; i += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], fmaxf(sc[i + e], sc[i + 4 + e]));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], sc[28 + e]);
-            const float top = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * scale;
-            // The maximum only takes whole values, so that what it moves is multiplied by powers of two.
-            const bool move = exists && top > m + kSlack;
-            if (__any_sync(0xffffffffu, move)) {
-              const float to = move ? ceilf(top) : m;
-              const float f = ex2(m - to);
-              m = to;
-              l *= f;
-              if (any) {  // O holds the tiles before this one: wait for the last of them
-                if (!wait(&B.pv_done[g][buf ^ 1], ((j - 1) >> 1) & 1u)) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int d = 0; d < HD; d += 16) {
-                  uint32_t o[16];
-                  tmem_ld_x16(obase + d, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_st_x16(obase + d, o);
+                for (int i = 0; i < 16; ++i) {
+                  const unsigned long long f = CODES ? reinterpret_cast<const unsigned long long*>(scales)[16 * h + i] : up;
+                  f2_unpack(f2_mul(f2_pack(sc[2 * i], sc[2 * i + 1]), f), sc[2 * i], sc[2 * i + 1]);
                 }
-                tmem_wait_st();
               }
-              // and the probabilities in front of these
+              uint32_t seen = 0xFFFFFFFFu;
+              if (partly) {
+                const int k0 = base + 32 * h;
+                seen = !exists ? 0u
+                               : first_bits(w.key1 - k0) & (a.mask == nullptr
+                                                                ? first_bits(w.ctx + node - k0 + 1)
+                                                                : mask_window(a.mask + token * a.mask_words, a.mask_words, k0 - w.ctx));
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!((seen >> i) & 1u)) sc[i] = -INFINITY;
+              }
+              float x4[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+              for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], fmaxf(sc[i + e], sc[i + 4 + e]));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x4[e] = fmaxf(x4[e], sc[28 + e]);
+              const float top = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * scale;
+              // The maximum only takes whole values, so that what it moves is multiplied by powers of two.
+              const bool move = exists && top > m + kSlack;
+              if (__any_sync(0xffffffffu, move)) {
+                const float to = move ? ceilf(top) : m;
+                const float f = ex2(m - to);
+                m = to;
+                l *= f;
+                if (any) {  // O holds the tiles before this one: wait for the last of them
+                  if (!wait(&B.pv_done[g][buf ^ 1], ((j - 1) >> 1) & 1u)) break;
+                  tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < 4 * h; ++c) {
-                uint4* q = reinterpret_cast<uint4*>(prow + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4));
-                uint32_t e[4] = {q->x, q->y, q->z, q->w};
+                  for (int d = 0; d < HD; d += 16) {
+                    uint32_t o[16];
+                    tmem_ld_x16(obase + d, o);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = pack_rn_bf16x2(bf16lo(e[i]) * f, bf16hi(e[i]) * f);
-                *q = make_uint4(e[0], e[1], e[2], e[3]);
-              }
-            }
-            unsigned long long sum = f2_pack(0.f, 0.f);
-            const unsigned long long scale2 = f2_pack(scale, scale), minus_m = f2_pack(-m, -m);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t e[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int k = 8 * c + 2 * i;
-                float p0, p1;
-                f2_unpack(f2_fma(f2_pack(sc[k], sc[k + 1]), scale2, minus_m), p0, p1);
-                p0 = ex2(p0);
-                p1 = ex2(p1);
-                sum = f2_add(sum, f2_pack(p0, p1));
-                if constexpr (CODES) {
-                  f2_unpack(f2_mul(f2_pack(p0, p1), reinterpret_cast<const unsigned long long*>(scales)[BK / 2 + 16 * h + k / 2]), p0, p1);
-                  if (partly) {  // (a hidden key's scale may be NaN)
-                    if (!((seen >> k) & 1u)) p0 = 0.f;
-                    if (!((seen >> (k + 1)) & 1u)) p1 = 0.f;
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st_x16(obase + d, o);
                   }
+                  tmem_wait_st();
                 }
-                e[i] = pack_rn_bf16x2(p0, p1);
+                // and the probabilities in front of these
+#pragma unroll 1
+                for (int c = 0; c < 4 * h; ++c) {
+                  uint4* q = reinterpret_cast<uint4*>(prow + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4));
+                  uint32_t e[4] = {q->x, q->y, q->z, q->w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) e[i] = pack_rn_bf16x2(bf16lo(e[i]) * f, bf16hi(e[i]) * f);
+                  *q = make_uint4(e[0], e[1], e[2], e[3]);
+                }
               }
-              *reinterpret_cast<uint4*>(prow + (h >> 1) * 16384 + (((4 * (h & 1) + c) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+              unsigned long long sum = f2_pack(0.f, 0.f);
+              const unsigned long long scale2 = f2_pack(scale, scale), minus_m = f2_pack(-m, -m);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int k = 8 * c + 2 * i;
+                  float p0, p1;
+                  f2_unpack(f2_fma(f2_pack(sc[k], sc[k + 1]), scale2, minus_m), p0, p1);
+                  p0 = ex2(p0);
+                  p1 = ex2(p1);
+                  sum = f2_add(sum, f2_pack(p0, p1));
+                  if constexpr (CODES) {
+                    f2_unpack(f2_mul(f2_pack(p0, p1), reinterpret_cast<const unsigned long long*>(scales)[BK / 2 + 16 * h + k / 2]), p0, p1);
+                    if (partly) {  // (a hidden key's scale may be NaN)
+                      if (!((seen >> k) & 1u)) p0 = 0.f;
+                      if (!((seen >> (k + 1)) & 1u)) p1 = 0.f;
+                    }
+                  }
+                  e[i] = pack_rn_bf16x2(p0, p1);
+                }
+                *reinterpret_cast<uint4*>(prow + (h >> 1) * 16384 + (((4 * (h & 1) + c) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+              }
+              float s0, s1;
+              f2_unpack(sum, s0, s1);
+              l += s0 + s1;
             }
-            float s0, s1;
-            f2_unpack(sum, s0, s1);
-            l += s0 + s1;
-          }
           }
           if (!ok) break;
         } else {
