@@ -635,7 +635,7 @@ NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, con
  * kv_heads at most 32768. Scores (taken to be above -1e30), softmax and sums are
  * f32; for their product with the values the probabilities are rounded to bf16,
  * or, over codes and up to 32 rows of a kv head, to f16 (the values' scales, not
- * negative, included; half a step is 2^-12 of a term or 2^-32 of the row's largest). A new token's key or value that is not finite reaches only
+ * negative, included; half a step is 2^-11 of a term or 2^-32 of the row's largest). A new token's key or value that is not finite reaches only
  * the nodes that see it. The
  * result does not depend on how the keys are split over the GPU beyond f32 rounding,
  * and is the same on every run. `workspace` (16-byte aligned device memory) of

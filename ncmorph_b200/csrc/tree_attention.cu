@@ -19,12 +19,12 @@
 // Codes are used as they are: int8 and e4m3 values are exact in f16, a key's
 // scale multiplies its scores, and a value's scale s enters its probability's
 // exponent, p' = 2^(t + log2 s - m'), with a maximum m' of its own. P is then f16,
-// which costs 2^-12 of each term, or 2^-32 of the row's largest (lifted by 2^7, the
-// largest is at 2^7 or above, and f16's steps end at 2^-24). Q is bf16 and becomes f16 with a power of two
-// of its row taken out; what is then below f16's range is 2^-30 of the
-// row's largest. A bf16 cache is multiplied in bf16 (its values do not fit f16's
-// range), with P rounded to bf16: 2^-9 of each term, about as much again as the output's
-// own rounding.
+// which costs 2^-11 of each term, or 2^-32 of the row's largest (lifted by 2^7, the
+// largest is at 2^7 or above, and f16's steps end at 2^-24). Q is bf16 and becomes
+// f16 with a power of two of its row taken out: exact, but for values below 2^-17 of
+// the row's largest, which are off by 2^-25 of that. A bf16 cache is multiplied in
+// bf16 (its values do not fit f16's range), with P rounded to bf16: 2^-8 of each
+// term, in a sum of many about as much again as the output's own rounding.
 //
 // A maximum is only moved when a score passes it by 2^8, so most tiles
 // neither reduce over lanes nor rescale.
@@ -35,9 +35,9 @@
 // sequences, int8: 34 us, 1.6 TB/s). A short context (4 sequences of 200 tokens) takes
 // 5.7 us: one launch, and a chain of four loads.
 //
-// Split: items are cut into units of unit_keys keys, and every CTA of one wave
-// takes the same number of consecutive units, whatever the sequences' lengths
-// are (they are known on the device only). A CTA that ends inside an item
+// Split: items are cut into units of 128 keys, and every CTA of one wave takes
+// the same number of consecutive units (beginning an item counts as three more),
+// whatever the sequences' lengths are: they are known on the device only. A CTA that ends inside an item
 // leaves its sums in the workspace: slot 2c for an item begun by an earlier
 // CTA, slot 2c + 1 for one that goes on in the next. tree_merge_kernel adds the
 // slots of such items up, in order.
