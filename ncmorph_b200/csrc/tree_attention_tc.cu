@@ -17,8 +17,8 @@
 //
 // Bound: the exponentials (16 a clock and SM: 64 keys of 128 rows take 512 clocks, the
 // two products 256 at head_dim 64 and 512 at 128). Two trees of 64 tokens over up to 131072
-// tokens, bf16, head_dim 64 (256 rows): 139 us, 525 TFLOP/s; the special-function unit
-// is busy 51 % of the kernel's time, and a group's 64 keys take 2000 clocks, 1024 of
+// tokens, bf16, head_dim 64 (256 rows): 136 us, 535 TFLOP/s; the special-function unit
+// is busy half of the kernel's time, and a group's 64 keys take 2000 clocks, 1024 of
 // them exponentials of both groups. Trees of 26 tokens of eight sequences of up to 8191 tokens, e4m3,
 // head_dim 128 (104 rows): 48 us, 179 TFLOP/s; a CTA has about ten tiles of each group there,
 // and its start (a chain of lookups and the first keys: 10000 clocks), the sums' way out and
@@ -39,8 +39,7 @@ constexpr int kLoadThreads = 32 * kLoadWarps;
 struct TcBars {
   uint64_t q_full;
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
-  uint64_t s_full[2][2], s_free[2][2];  // [group][buffer]
-  uint64_t p_full[2][2], pv_done[2][2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [group][buffer]
   uint64_t sums_full[4], taken[4];  // [pair of the groups' warps] their sums are there; both have read both groups' values
   uint64_t drain[2];
   uint32_t tmem_base;
@@ -167,7 +166,6 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
     for (int g = 0; g < 2; ++g)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&B.s_full[g][i], 1);
-        mbar_init(&B.s_free[g][i], 4);
         mbar_init(&B.p_full[g][i], 4);
         mbar_init(&B.pv_done[g][i], 1);
       }
@@ -281,12 +279,6 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
                 f2_unpack(f2_fma(f2_pack(sc[2 * i], sc[2 * i + 1]), f, minus_m), sc[2 * i], sc[2 * i + 1]);
                 worst = fmaxf(worst, fmaxf(sc[2 * i], sc[2 * i + 1]));
               }
-              if (h == BK / 16 - 1) {
-                if (__any_sync(0xffffffffu, exists && worst > kSlack)) return false;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
-              }
               if (h == 0 && !p_free()) {
                 tmem_wait_ld();
                 return true;
@@ -310,6 +302,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
                 *reinterpret_cast<uint4*>(prow + (h >> 2) * 16384 + (((2 * (h & 3) + c) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
               }
             }
+            if (__any_sync(0xffffffffu, exists && worst > kSlack)) return false;
             float s0, s1;
             f2_unpack(f2_add(sum, sum2), s0, s1);
             l += s0 + s1;
@@ -329,11 +322,6 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
               float* sc = reinterpret_cast<float*>(raw);
               tmem_ld_x32(sbase + 32 * h, raw);
               tmem_wait_ld();
-              if (h == BK / 32 - 1) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
-              }
               if (!late) {
                 const unsigned long long up = f2_pack(a.scale_log2, a.scale_log2);
 #pragma unroll
@@ -422,8 +410,6 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
             }
           }
           if (!ok) break;
-        } else {
-          if (lane == 0) mbar_arrive(&B.s_free[g][buf]);
         }
         any = true;
         tc_fence_before();
@@ -547,7 +533,8 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       uint32_t js = 0, jo = 0, segment = 0;  // products issued, of each kind
       bool ok = true;
       auto s_ready = [&](uint32_t n) {
-        return mbar_test_wait(&B.k_full[n % NS], (n / NS) & 1u) && (js < 2 || mbar_test_wait(&B.s_free[g][js & 1], ((js - 2) >> 1) & 1u));
+        // (P of the tile two before is there when its product was issued: so its scores were read)
+        return js < jo + 2 && mbar_test_wait(&B.k_full[n % NS], (n / NS) & 1u);
       };
       auto issue_s = [&](uint32_t n) {
         const uint32_t st = n % NS, buf = js & 1u;
@@ -592,7 +579,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         uint64_t since = 0;
         uint32_t tries = 0;
         while (ok && no < number) {
-          if (ns < number && js < jo + 2 && s_ready(ns)) {
+          if (ns < number && s_ready(ns)) {
             issue_s(ns);
             ns += STEP;
           } else if (no < ns && pv_ready(no)) {
