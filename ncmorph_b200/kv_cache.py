@@ -110,16 +110,23 @@ def gather(cache: KVCache, row_start: torch.Tensor, page_table: torch.Tensor, ro
     row_start[b] + i is position begin[b] + i of sequence b (begin None: 0).
     out_k / out_v may be column slices of wider rows (fused QKV rows for
     ncm_model.attention_bf16); without them `rows` says how many to make."""
-    dev = cache.device
-    if out_k is None or out_v is None:
-        if rows is None:
+    dev, width = cache.device, cache.width
+    if rows is None:
+        if out_k is None or out_v is None:
             raise ValueError("rows is needed without out_k and out_v")
-        out_k = empty_rows(rows, cache.width, bf16, dev) if out_k is None else out_k
-        out_v = empty_rows(rows, cache.width, bf16, dev) if out_v is None else out_v
-    ks, vs = need_rows(out_k, bf16, "out_k", dev, cache.width), need_rows(out_v, bf16, "out_v", dev, cache.width)
-    if out_v.shape[0] != out_k.shape[0] or (rows is not None and out_k.shape[0] != rows):
+        rows = out_k.shape[0] if isinstance(out_k, torch.Tensor) and out_k.dim() == 2 else 0
+    ks = vs = width
+    if out_k is None:
+        out_k = empty_rows(rows, width, bf16, dev)
+    else:
+        ks = need_rows(out_k, bf16, "out_k", dev, width)
+    if out_v is None:
+        out_v = empty_rows(rows, width, bf16, dev)
+    else:
+        vs = need_rows(out_v, bf16, "out_v", dev, width)
+    if out_k.shape[0] != rows or out_v.shape[0] != rows:
         raise ValueError("out_k and out_v must have the same rows")
-    b = _batch(cache, row_start, None, page_table, out_k.shape[0])
+    b = _batch(cache, row_start, None, page_table, rows)
     _lib.call("ncm_kv_cache_gather", context_of(dev), cache._ref, ctypes.byref(b),
               need_vec(begin, i32, "begin", dev, b.batch), out_k.data_ptr(), ks, out_v.data_ptr(), vs, raw_stream(dev))
     return out_k, out_v

@@ -840,6 +840,12 @@ def test_refusals(cuda_dev):
         kv_cache.KVCache(cache.k, cache.v)
     with pytest.raises(ValueError):
         kv_cache.gather(cache, start, table)
+    for wrong in (dict(out_k=bf(1, 128), out_v=bf(2, 128)), dict(rows=2, out_k=bf(1, 128)), dict(rows=2, out_v=bf(1, 128)),
+                  dict(out_k=bf(1, 128)), dict(out_k=bf(1, 64), out_v=bf(1, 128)), dict(rows=-1)):
+        with pytest.raises((ValueError, RuntimeError)):
+            kv_cache.gather(cache, start, table, **wrong)
+    with pytest.raises(TypeError):
+        kv_cache.gather(cache, start, table, out_k=[1], out_v=bf(1, 128))
     with pytest.raises(_lib.NcmError):  # three heads over two kv heads
         kv_cache.tree_attention(bf(1, 192), cache, start, lens, table, max_nodes=1)
     with pytest.raises(_lib.NcmError):
