@@ -157,7 +157,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     words = 0
     if tree_mask is not None:
         if not isinstance(tree_mask, torch.Tensor) or tree_mask.dim() != 2 or tree_mask.dtype != i32 or \
-                tree_mask.device != dev or tree_mask.shape[0] != T or not tree_mask.is_contiguous():
+                tree_mask.device != dev or tree_mask.shape[0] != T or not tree_mask.is_contiguous() or \
+                tree_mask.shape[1] < 1:  # (an empty mask has no address, and would be none)
             raise ValueError(f"tree_mask must be a contiguous int32 [{T}, words] tensor on {dev}")
         words = tree_mask.shape[1]
     if out is None:

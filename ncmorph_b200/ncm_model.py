@@ -343,6 +343,8 @@ def process_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, tok
         r.allowed_stride = need_rows(allowed, i32, "allowed", dev, (V + 31) // 32)
         r.allowed = allowed.data_ptr()
         r.allowed_count = allowed.shape[0]
+        if r.allowed_count == 0 and R > 0:
+            raise ValueError("allowed must hold at least one mask")
         r.allowed_rows = need_vec(allowed_rows, i32, "allowed_rows", dev, R)
     elif allowed_rows is not None:
         raise ValueError("allowed_rows needs allowed")

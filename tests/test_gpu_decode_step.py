@@ -1029,6 +1029,11 @@ def test_refusals_of_sizes(cuda_dev):
         kv_cache.tree_attention(bf(64), cache, start, lens, table, max_nodes=1)
     with pytest.raises(ValueError):
         kv_cache.tree_attention(bf(1, 64), cache, start, lens, table, max_nodes=1, tree_mask=[[1]])
+    with pytest.raises(ValueError):  # a mask without words is not a chain
+        kv_cache.tree_attention(bf(1, 64), cache, start, lens, table, max_nodes=1, tree_mask=torch.zeros((1, 0), dtype=torch.int32, device=cuda_dev))
+    with pytest.raises(ValueError):
+        ncm_model.process_logits(torch.zeros((1, 32), device=cuda_dev), allowed=torch.zeros((0, 1), dtype=torch.int32, device=cuda_dev),
+                                 allowed_rows=i32(0))
     with pytest.raises(_lib.NcmError):
         kv_cache.tree_attention(bf(1, 64), cache, start, lens, table, max_nodes=1, tree_mask=torch.zeros((1, 33), dtype=torch.int32, device=cuda_dev))
     for shape in ((4, 1, 16, 96), (4, 1, 24, 64), (4, 1, 4, 64), (4, 1, 2048, 64)):
