@@ -425,7 +425,6 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       // rows, a row's values lie in the same lane of tensor memory: each group adds
       // up half of the columns.
       const bool whole = w.whole();
-      const bool odd = !CODES && *const_cast<volatile int*>(&B.odd_values) != 0;
       constexpr int COLS = SPLITQ ? HD : HD / 2;
       const int d0 = SPLITQ ? 0 : g * COLS;
       float f0 = 1.f, f1 = 0.f;  // weights of this group's and the other one's values
@@ -445,6 +444,9 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
         l = fmaf(x.y, f0, y.y * f1);
         two = ntiles > 1;  // (otherwise the second group had nothing)
       }
+      // (behind the wait for the other group's sums: a group has waited for its own tiles only, and
+      // writes columns of both groups' values)
+      const bool odd = !CODES && *const_cast<volatile int*>(&B.odd_values) != 0;
       float* part = a.part + ((2ll * blockIdx.x + (w.u0 == 0 ? 1 : 0)) * ROWS + qt * 128 + row) * (HD + 4);
       uint16_t* out = a.out + token * a.out_stride + head * HD;
       const uint32_t o0 = SPLITQ ? obase : tmem + lanes + 256;

@@ -1076,3 +1076,31 @@ def test_no_history_yet(cuda_dev):
     args["tokens"], args["token_start"] = i32(), i32(0, 0, 1)  # a bound past the (empty) list
     assert torch.equal(ncm_model.process_logits(x, **args), x)
     expect_range_error(cuda_dev)
+
+
+@pytest.mark.parametrize("n,L,hd,heads", [(40, 50, 64, 1), (40, 50, 128, 1), (40, 64, 64, 1), (20, 800, 128, 4), (40, 193, 64, 1),
+                                          (33, 257, 128, 1), (40, 1100, 64, 1), (60, 449, 128, 2), (64, 600, 64, 4)])
+def test_infinite_values_in_the_last_tile(cuda_dev, n, L, hd, heads):
+    """Values that are not finite in the very last new tokens only, in every 16th column:
+    a softmax group that never waited for that tile writes half of the columns."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, torch.bfloat16, [L, L - 1], [n, n], 1, hd, 16, seed=n + L)
+    want = torch.zeros((n, hd), dtype=torch.bool)
+    for end in (L, 2 * L - 1):
+        w.v[end - 2, ::16], w.v[end - 1, 8::16] = math.inf, -math.inf
+    want[n - 2:, ::16], want[n - 1:, 8::16] = True, True
+    want = want.repeat(2, heads)
+    w.fill()
+    q = torch.randn((2 * n, heads * hd), generator=w.g).to(torch.bfloat16)
+    args = (q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table)
+    out, lse = kv_cache.tree_attention(*args, max_nodes=n, return_lse=True)
+    for _ in range(20):
+        again, lse2 = kv_cache.tree_attention(*args, max_nodes=n, return_lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    out = out.cpu()
+    assert torch.equal(torch.isinf(out), want) and not torch.isnan(out).any()
+    up = torch.arange(hd).repeat(heads) % 16 == 0
+    assert torch.all(out[:, up][want[:, up]] > 0) and torch.all(out[:, ~up][want[:, ~up]] < 0)
+    w.v[~torch.isfinite(w.v)] = 0.0
+    o, l, to, tl = attend_ref(w, q, heads, None, hd ** -0.5)
+    assert torch.all(((out.double() - o).abs() <= to) | want) and torch.all((lse.cpu().double() - l).abs() <= tl)
