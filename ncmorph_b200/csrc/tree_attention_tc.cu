@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&B.q_full, 4 * S::kQTiles);
+    mbar_init(&B.q_full, 4 * S::kQTiles + 2);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&B.k_full[i], kLoadWarps);
       mbar_init(&B.v_full[i], kLoadWarps);
@@ -565,6 +565,9 @@ __global__ void __launch_bounds__(TcShape<HD, FMT, SPLITQ>::kThreads, 1) tree_at
       for (; ok && w.next(a); ++segment) {
         const uint32_t ntiles = (w.key1 - w.key0 + BK - 1) / BK, n0 = number;
         number += ntiles;
+        // (arrives as well as waits: a group without products in this segment would otherwise not be
+        // waited for by anyone, and two segments late take one phase for another)
+        mbar_arrive(&B.q_full);
         if (!(ok = tc_wait(&B.q_full, segment & 1u, abort_flag))) break;
         if (SPLITQ && w.live_rows <= 128 * g) {  // no rows: the tiles are only given back
           for (uint32_t n = n0; ok && n < number; ++n) {

@@ -1104,3 +1104,28 @@ def test_infinite_values_in_the_last_tile(cuda_dev, n, L, hd, heads):
     w.v[~torch.isfinite(w.v)] = 0.0
     o, l, to, tl = attend_ref(w, q, heads, None, hd ** -0.5)
     assert torch.all(((out.double() - o).abs() <= to) | want) and torch.all((lse.cpu().double() - l).abs() <= tl)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("most,heads,hd", [(40, 4, 64), (12, 16, 128), (50, 16, 64), (60, 8, 128)])
+@pytest.mark.parametrize("split", [False, True])
+def test_many_items_of_many_rows(cuda_dev, dtype, most, heads, hd, split):
+    """Several times as many items as the tcgen05 kernel has CTAs: runs of segments of one
+    tile among longer ones, odd and even tile counts, sequences without new tokens and
+    ones that leave warps, or one group of 128 rows, without any row."""
+    from ncmorph_b200 import kv_cache
+    g = torch.Generator().manual_seed(most * heads)
+    lens = [int(x) for x in torch.randint(1, 201, (130,), generator=g)]
+    lens[20:60] = [1 + (7 * b) % 64 for b in range(40)]
+    if split:  # long ones are shared by several CTAs
+        lens[70], lens[129] = 1537, 3000
+    new = [min(n, int(x)) for n, x in zip(lens, torch.randint(0, most + 1, (130,), generator=g))]
+    new[25:45] = [min(n, 1 + b % 3) for b, n in enumerate(lens[25:45])]
+    w = World(cuda_dev, dtype, lens, new, 4, hd, 16, seed=most).fill()
+    q = torch.randn((w.T, heads * hd), generator=w.g).to(torch.bfloat16)
+    sees, bits = tree_masks(new, w.g)
+    args = (q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table)
+    out, lse = kv_cache.tree_attention(*args, max_nodes=most, tree_mask=bits.to(cuda_dev), return_lse=True)
+    again, _ = kv_cache.tree_attention(*args, max_nodes=most, tree_mask=bits.to(cuda_dev), return_lse=True)
+    assert torch.equal(out, again)
+    check_attention(out, lse, attend_ref(w, q, heads, sees, hd ** -0.5))
