@@ -27,7 +27,8 @@
 // term, in a sum of many about as much again as the output's own rounding.
 //
 // A maximum is only moved when a score passes it by 2^8, so most tiles
-// neither reduce over lanes nor rescale.
+// neither reduce over lanes nor rescale. It only takes whole values: what a row's keys
+// were split into changes its probabilities by powers of two, not their 16-bit rounding.
 //
 // Bound: the cache's bytes with few rows (single tokens of 32 sequences of up to
 // 32768 tokens, 32 query over 8 kv heads of 64, int8: 70 us, 5.6 TB/s, 0.85 of a
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
             float x = top[nt][e];
 #pragma unroll
             for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
-            x = fmaxf(x, m[nt][e]);
+            x = fmaxf(ceilf(x), m[nt][e]);
             float f = ex2(m[nt][e] - x);
             m[nt][e] = x;
             l[nt][e] *= f;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
               x = topv[nt][e];
 #pragma unroll
               for (int z = 4; z < 32; z <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
-              x = fmaxf(x - kLift, mv[nt][e]);
+              x = fmaxf(floorf(x - kLift), mv[nt][e]);
               f = ex2(mv[nt][e] - x);
               mv[nt][e] = x;
             }

@@ -1129,3 +1129,28 @@ def test_many_items_of_many_rows(cuda_dev, dtype, most, heads, hd, split):
     again, _ = kv_cache.tree_attention(*args, max_nodes=most, tree_mask=bits.to(cuda_dev), return_lse=True)
     assert torch.equal(out, again)
     check_attention(out, lse, attend_ref(w, q, heads, sees, hd ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("n", [1, 5])
+def test_split_changes_no_rounding_of_probabilities(cuda_dev, dtype, n):
+    """A sequence alone and among others: its keys are dealt out differently, and maxima
+    move by powers of two only, so the 16-bit probabilities stay.
+
+    Scores have the same bits. A probability is 2^(t - m), whose difference of up to 2^4 is
+    rounded by 2^-21: 2^-20 apart, relative to itself, in two splits, so it falls on two sides
+    of a border of its rounding (steps of 2^-8 or, over codes, 2^-11, relative to it) with a chance
+    of 2^-12 or 2^-9, and is then a step off. For an output, a sum of many of random signs,
+    that is sqrt(2^-12) 2^-8 or sqrt(2^-9) 2^-11 of itself, about 2^-14 or 2^-15.5; the f32 sums'
+    order is below that. It takes another bf16 (steps of 2^-8 to 2^-7) with a chance of 1.6 % or 0.6 %.
+    Probabilities rounded independently are 2^-9.3 (2^-12.3) apart: 40 % or 5 %."""
+    from ncmorph_b200 import kv_cache
+    lens = [1700, 2950, 300, 2100, 40, 900, 3500, 128, 1300, 2600, 777, 1500, 64]
+    w = World(cuda_dev, dtype, lens, [n] * len(lens), 8, 64, 16, seed=n).fill()
+    q = torch.randn((w.T, 32 * 64), generator=w.g).to(torch.bfloat16).to(cuda_dev)
+    out, lse = kv_cache.tree_attention(q, w.cache, w.start, w.kv_lens, w.table, max_nodes=n, return_lse=True)
+    alone, lse2 = kv_cache.tree_attention(q[:4 * n].contiguous(), w.cache, w.starts([n] * 4), w.kv_lens[:4].contiguous(),
+                                          w.table[:4].contiguous(), max_nodes=n, return_lse=True)
+    share = float((out[:4 * n] != alone).float().mean())
+    assert share <= (0.08 if dtype == torch.bfloat16 else 0.025), share
+    assert torch.all((lse[:4 * n] - lse2).abs() <= 2.0 ** -18 * (1 + lse2.abs()))
