@@ -152,6 +152,19 @@ class DeviceFlags {
   std::atomic<unsigned long long> bits_{0};
 };
 
+// A number of each device that is asked for once (CTAs of a kernel on one SM, say).
+// 0: not asked yet, and always so past 64 devices.
+class DeviceNumbers {
+ public:
+  int get(int dev) const { return dev >= 0 && dev < 64 ? numbers_[dev].load(std::memory_order_acquire) : 0; }
+  void set(int dev, int number) {
+    if (dev >= 0 && dev < 64) numbers_[dev].store(number, std::memory_order_release);
+  }
+
+ private:
+  std::atomic<int> numbers_[64] = {};
+};
+
 // Makes a context's device current for one entry point and puts the calling
 // thread's device back when it returns.
 class DeviceGuard {

@@ -748,14 +748,13 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
     return ncm_fail(NCM_EINVAL, "%s: too many sequences", what);
   int index = 0;
   p->v = pick(cache, static_cast<int64_t>(max_nodes) * (heads / cache->kv_heads), &index);
-  static std::atomic<int> resident[3 * 2 * (kSizes + 2)];  // CTAs of a variant on one SM
-  static DeviceFlags ready[3 * 2 * (kSizes + 2)];
-  if (!ready[index].test(ctx->device)) {
-    int n = 0;
+  static DeviceNumbers resident[3 * 2 * (kSizes + 2)];  // CTAs of a variant on one SM of a device
+  int on_sm = resident[index].get(ctx->device);
+  if (on_sm == 0) {
     NCM_CUDA_TRY(cudaFuncSetAttribute(p->v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p->v.smem));
-    NCM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, p->v.kernel, p->v.threads, p->v.smem));
-    resident[index].store(std::max(1, n));
-    ready[index].set(ctx->device);
+    NCM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&on_sm, p->v.kernel, p->v.threads, p->v.smem));
+    on_sm = std::max(1, on_sm);
+    resident[index].set(ctx->device, on_sm);
   }
   const int64_t cap = std::min<int64_t>(static_cast<int64_t>(batch->table_width) * cache->page_size, 1 << 30);
   p->merge = cap > 1 << kWholeShift;
@@ -764,7 +763,7 @@ int tree_plan(ncm_ctx* ctx, const char* what, const ncm_kv_cache_t* cache, const
   // (the kernels multiply the number of units by that of the CTAs)
   if (batch->batch * cache->kv_heads * tiles * (kBeginCost + ceil_div(cap, 1 << p->unit_shift)) > INT64_MAX / (2 * kMaxParts))
     return ncm_fail(NCM_EINVAL, "%s: too many keys", what);
-  p->grid = std::min(kMaxParts, ctx->num_sms * resident[index].load());
+  p->grid = std::min(kMaxParts, ctx->num_sms * on_sm);
   p->bytes = static_cast<uint64_t>(2) * p->grid * p->v.rows * (cache->head_dim + 4) * sizeof(float);
   return NCM_OK;
 }

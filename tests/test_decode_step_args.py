@@ -1,10 +1,12 @@
 """Arguments that the decode-step operators refuse before any device is touched."""
 import ctypes
+import pathlib
+import subprocess
 
 import pytest
 import torch
 
-from ncmorph_b200 import _lib, kv_cache, ncm_model
+from ncmorph_b200 import _lib, build, kv_cache, ncm_model
 
 BF = torch.bfloat16
 
@@ -45,3 +47,24 @@ def test_struct_sizes_are_the_headers():
     assert ctypes.sizeof(_lib.KvCache) == 4 * 8 + 4 * 4 + 8
     assert ctypes.sizeof(_lib.KvBatch) == 3 * 8 + 8 + 2 * 4 + 8
     assert ctypes.sizeof(_lib.LogitRules) == 15 * 8
+
+
+def test_numbers_of_devices_stay_apart(tmp_path):
+    """The attention's plan keeps its CTAs per SM by device: what another device answers
+    must not change the workspace that a caller has been told."""
+    csrc = pathlib.Path(_lib.__file__).parent / "csrc"
+    program = tmp_path / "numbers.cu"
+    program.write_text('''#include "internal.h"
+int main() {
+  static ncm::DeviceNumbers n;
+  if (n.get(0) != 0 || n.get(63) != 0) return 1;
+  n.set(0, 4);
+  n.set(63, 2);
+  n.set(64, 9);
+  n.set(-1, 9);
+  return n.get(0) == 4 && n.get(63) == 2 && n.get(1) == 0 && n.get(64) == 0 && n.get(-1) == 0 ? 0 : 2;
+}
+''')
+    subprocess.run([build.nvcc(), "-std=c++17", f"-I{csrc}", f"-I{csrc.parents[1] / 'include'}", str(program), "-o", str(tmp_path / "numbers")],
+                   check=True)
+    assert subprocess.run([str(tmp_path / "numbers")]).returncode == 0
