@@ -171,6 +171,19 @@ __device__ __forceinline__ int slot_of_row(const RowsArgs& a, long long t) {
   return (page << a.pools.page_shift) + (pos & ((1 << a.pools.page_shift) - 1));
 }
 
+// Reports sequences that no row of the call leads to, but whose rows are not there: past the
+// end, or fewer than none. By threads that have no slot to look up, while others do.
+__device__ __forceinline__ void check_sequences(const RowsArgs& a) {
+  constexpr unsigned kCheckers = kRowThreads - 32;
+  if (blockIdx.y != 0 || threadIdx.x < 32) return;
+  const int rows = static_cast<int>(a.batch.rows);
+#pragma unroll 1
+  for (unsigned b = blockIdx.x * kCheckers + threadIdx.x - 32; b < static_cast<unsigned>(a.batch.batch); b += gridDim.x * kCheckers) {
+    const int first = __ldg(a.batch.token_start + b), end = __ldg(a.batch.token_start + b + 1);
+    if (end < first || (end > first && (first < 0 || end > rows))) atomicOr(a.err, kErrBadIndex);
+  }
+}
+
 // A block moves chunks of `tokens` rows: one lane each resolves the next chunk's
 // slots while this one's rows are on their way. A thread keeps its eight values
 // of a row (a head of the keys or the values: blockIdx.y picks the part of the
@@ -194,6 +207,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_rows_kernel(const RowsArgs a) 
   long long t0 = static_cast<long long>(blockIdx.x) * a.tokens;
   const long long t_step = static_cast<long long>(gridDim.x) * a.tokens;
   if (threadIdx.x < a.tokens) slot_of[0][threadIdx.x] = slot_of_row<APPEND>(a, t0 + threadIdx.x);
+  check_sequences(a);
   __syncthreads();
   for (int turn = 0; t0 < a.batch.rows; t0 += t_step, turn ^= 1) {
     const int* slots = slot_of[turn];

@@ -1154,3 +1154,29 @@ def test_split_changes_no_rounding_of_probabilities(cuda_dev, dtype, n):
     share = float((out[:4 * n] != alone).float().mean())
     assert share <= (0.08 if dtype == torch.bfloat16 else 0.025), share
     assert torch.all((lse[:4 * n] - lse2).abs() <= 2.0 ** -18 * (1 + lse2.abs()))
+
+
+@pytest.mark.parametrize("start,n", [([0, 3, 5], 3), ([0, 2, 1], 2), ([0, 3, -2], 3), ([3, 3, 9], 0)])
+def test_sequences_that_no_row_leads_to(cuda_dev, start, n):
+    """The second sequence's rows are past the end, or fewer than none: reported, although
+    the call has no row of it; the first one's n rows are written and read."""
+    from ncmorph_b200 import device, kv_cache
+    w = World(cuda_dev, torch.bfloat16, [20, 20], [1, 1], 1, 64, 16).fill()
+    rows = torch.randn((3, 64), generator=w.g).to(torch.bfloat16).to(cuda_dev)
+    starts = torch.tensor(start, dtype=torch.int32, device=cuda_dev)
+    before = w.cache.k.clone()
+    kv_cache.append(w.cache, rows, rows, starts, w.kv_lens, w.table)
+    expect_range_error(cuda_dev)
+    assert int((w.cache.k.view(torch.int16) != before.view(torch.int16)).any(-1).sum()) == n
+    out = torch.full((3, 64), 3.0, device=cuda_dev).to(torch.bfloat16)
+    kv_cache.gather(w.cache, starts, w.table, out_k=out, out_v=out.clone())
+    expect_range_error(cuda_dev)
+    assert torch.all(out[n:] == 3.0) and not torch.any((out[:n] == 3.0).all(-1))
+    # one of many sequences, whose other numbers are those of empty ones
+    at = torch.zeros(602, dtype=torch.int32, device=cuda_dev)
+    lens, table = torch.zeros(601, dtype=torch.int32, device=cuda_dev), torch.zeros((601, 1), dtype=torch.int32, device=cuda_dev)
+    kv_cache.append(w.cache, rows[:1], rows[:1], at, lens, table)
+    device.sync(cuda_dev)
+    at[451:] = -1
+    kv_cache.append(w.cache, rows[:1], rows[:1], at, lens, table)
+    expect_range_error(cuda_dev)
