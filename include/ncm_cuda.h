@@ -549,7 +549,7 @@ NCM_API int ncm_rvq_level_noalloc_status(ncm_stream_t stream, int32_t* flags);
  * packages/kernels/root.zig:615-633; ncm_attention_bf16 keeps that). `inverse`
  * rotates by the negative angle: the gradient of the forward rotation.
  * Columns rotary_dim .. head_dim are copied. y may be x with the same
- * stride (in place); where else the two ranges of rows overlap, column slices of
+ * stride (in place; a single row has none); where else the two ranges of rows overlap, column slices of
  * one buffer included, the call is refused. A position outside
  * [0, table_rows) makes ncm_sync report NCM_ERANGE and leaves its row
  * unwritten. rotary_dim even, <= head_dim <= 1024; any alignment of whole elements. */
@@ -684,7 +684,7 @@ typedef struct ncm_logit_rules {
 /* out = the rules applied to logits [rows, vocab] (NCM_DTYPE_F32 or
  * NCM_DTYPE_BF16, row strides in elements), computed in f32. out_dtype is
  * NCM_DTYPE_F32, or NCM_DTYPE_BF16 for bf16 logits. out may be logits (same type and
- * stride: in place); other overlaps are refused. At most 65535 rows. Rows are
+ * stride, which a single row has not: in place); other overlaps are refused. At most 65535 rows. Rows are
  * what ncm_tied_head_logits or a language-model head wrote. */
 NCM_API int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dtype, int64_t stride, void* out,
                                int32_t out_dtype, int64_t out_stride, int64_t rows, int64_t vocab,

@@ -290,7 +290,7 @@ extern "C" int ncm_logits_process(ncm_ctx_t* ctx, const void* logits, int32_t dt
   if (rows == 0) return NCM_OK;
   if (!logits || !out || !aligned_to(logits, isz) || !aligned_to(out, osz))
     return ncm_fail(NCM_EINVAL, "logits_process: null or misaligned logits");
-  const bool in_place = logits == out && dtype == out_dtype && stride == out_stride;
+  const bool in_place = logits == out && dtype == out_dtype && (stride == out_stride || rows == 1);
   if (!in_place && ranges_overlap(logits, isz * ((rows - 1) * stride + vocab), out, osz * ((rows - 1) * out_stride + vocab)))
     return ncm_fail(NCM_EINVAL, "logits_process: logits and out overlap without being the same rows");
   LogitArgs a{logits, out, stride, out_stride, vocab, r, ctx->d_err};

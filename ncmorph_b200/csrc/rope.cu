@@ -169,7 +169,7 @@ extern "C" int ncm_rope_bf16(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride
   if (!aligned_to(x, 2) || !aligned_to(y, 2) || !aligned_to(positions, 4) || !aligned_to(cos_t, 4) ||
       !aligned_to(sin_t, 4))
     return ncm_fail(NCM_EINVAL, "rope: misaligned buffer");
-  const bool in_place = x == y && x_stride == y_stride;
+  const bool in_place = x == y && (x_stride == y_stride || T == 1);  // (a single row's stride says nothing)
   if (!in_place && ranges_overlap(x, 2 * ((T - 1) * x_stride + width), y, 2 * ((T - 1) * y_stride + width)))
     return ncm_fail(NCM_EINVAL, "rope: x and y overlap without being the same rows");
   RopeArgs a{};

@@ -1180,3 +1180,25 @@ def test_sequences_that_no_row_leads_to(cuda_dev, start, n):
     at[451:] = -1
     kv_cache.append(w.cache, rows[:1], rows[:1], at, lens, table)
     expect_range_error(cuda_dev)
+
+
+def test_single_rows_in_place_with_any_stride(cuda_dev):
+    """One row's stride says nothing: two views of one row are the same row."""
+    from ncmorph_b200 import ncm_model
+    cos, sin = tables(9, 64, cuda_dev)
+    pos = torch.tensor([7], dtype=torch.int32, device=cuda_dev)
+    row = torch.randn(5 * 64, device=cuda_dev).to(torch.bfloat16)
+    x, out = row.unsqueeze(0), row[:3 * 64].unsqueeze(0)
+    assert x.stride(0) != out.stride(0)
+    want = ncm_model.rope_bf16(x, pos, cos, sin, 3, 64)
+    rest = row[3 * 64:].clone()
+    ncm_model.rope_bf16(x, pos, cos, sin, 3, 64, out=out)
+    assert torch.equal(out, want) and torch.equal(row[3 * 64:], rest)
+    buf = torch.randn(40, device=cuda_dev)
+    logits, out = torch.as_strided(buf, (1, 33), (40, 1)), torch.as_strided(buf, (1, 33), (48, 1))
+    toks, at = torch.tensor([3, 3, 32], dtype=torch.int32, device=cuda_dev), torch.tensor([0, 3], dtype=torch.int32, device=cuda_dev)
+    pen = torch.tensor([0.5], device=cuda_dev)
+    want = ncm_model.process_logits(logits, toks, at, frequency=pen)
+    tail = buf[33:].clone()
+    ncm_model.process_logits(logits, toks, at, frequency=pen, out=out)
+    assert torch.equal(out, want) and torch.equal(buf[33:], tail)
