@@ -605,8 +605,8 @@ typedef struct ncm_kv_batch {
  * nearest, ties to even, exactly as in real arithmetic; A = 0 stores zeros
  * with scale 1, and a row holding a NaN or an infinity stores zeros with scale
  * NaN (it reads back as NaN). The e4m3 codes 0x7F and 0xFF are never stored, and
- * what the functions below make of them is not specified. Two positions that the page tables map to one
- * slot leave one of the two there, and not always the same one. */
+ * what the functions below make of them is not specified. Two positions of a call that the page tables map to one
+ * slot leave pieces of either there, unless their rows are equal. */
 NCM_API int ncm_kv_cache_append(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                 const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
                                 ncm_stream_t stream);
@@ -615,7 +615,8 @@ NCM_API int ncm_kv_cache_append(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, con
  * sequence b is position begin[b] + i (begin NULL: 0), i < token_start[b + 1] -
  * token_start[b]; batch->kv_lens is not used (may be NULL). k and v rows as in
  * ncm_kv_cache_append: with the K and V columns of fused QKV rows as targets
- * they are ncm_attention_bf16's operands. */
+ * they are ncm_attention_bf16's operands. Rows of k and v that overlap each other are
+ * refused, and so are rows that overlap a pool, here and in ncm_kv_cache_append. */
 NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                 const int32_t* begin, uint16_t* k, int64_t k_stride, uint16_t* v, int64_t v_stride,
                                 ncm_stream_t stream);

@@ -278,6 +278,15 @@ int launch_rows(ncm_ctx* ctx, const ncm_kv_cache_t* c, RowsArgs& a, cudaStream_t
   return NCM_OK;
 }
 
+// Whether row arrays a and b of equal width share an element (strides in elements). Column
+// slices of the same rows do not; other strides than each other's over one range are taken to.
+bool rows_overlap(const uint16_t* a, int64_t a_stride, const uint16_t* b, int64_t b_stride, int64_t rows, int64_t width) {
+  if (!ranges_overlap(a, 2 * ((rows - 1) * a_stride + width), b, 2 * ((rows - 1) * b_stride + width))) return false;
+  if (a_stride != b_stride) return true;
+  const int64_t at = (a < b ? b - a : a - b) % a_stride;
+  return at < width || at + width > a_stride;
+}
+
 int rows_args(const char* what, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, bool need_lens,
               const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride, RowsArgs* a) {
   int rc = kv_check_cache(what, cache);
@@ -286,6 +295,11 @@ int rows_args(const char* what, const ncm_kv_cache_t* cache, const ncm_kv_batch_
   if ((rc = kv_check_rows(what, "k", k, k_stride, batch->rows, width)) ||
       (rc = kv_check_rows(what, "v", v, v_stride, batch->rows, width)))
     return rc;
+  const size_t pool = static_cast<size_t>(cache->num_pages) * cache->page_size * width * (cache->format == NCM_KV_BF16 ? 2 : 1);
+  for (const void* p : {cache->k, cache->v})
+    if (batch->rows > 0 && (ranges_overlap(k, 2 * ((batch->rows - 1) * k_stride + width), p, pool) ||
+                            ranges_overlap(v, 2 * ((batch->rows - 1) * v_stride + width), p, pool)))
+      return ncm_fail(NCM_EINVAL, "%s: the rows overlap a pool", what);
   a->pools = kv_pools_of(cache);
   a->batch = kv_batch_of(batch);
   a->k = const_cast<uint16_t*>(k);
@@ -320,6 +334,8 @@ int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_k
   int rc = rows_args("kv_cache_gather", cache, batch, false, k, k_stride, v, v_stride, &a);
   if (rc || batch->batch == 0 || batch->rows == 0) return rc;
   if (!aligned_to(begin, 4)) return ncm_fail(NCM_EINVAL, "kv_cache_gather: misaligned begin");
+  if (rows_overlap(k, k_stride, v, v_stride, batch->rows, static_cast<int64_t>(cache->kv_heads) * cache->head_dim))
+    return ncm_fail(NCM_EINVAL, "kv_cache_gather: the rows of k and v overlap");
   a.begin = begin;
   return launch_rows<false>(ctx, cache, a, static_cast<cudaStream_t>(stream));
 }

@@ -1202,3 +1202,39 @@ def test_single_rows_in_place_with_any_stride(cuda_dev):
     tail = buf[33:].clone()
     ncm_model.process_logits(logits, toks, at, frequency=pen, out=out)
     assert torch.equal(out, want) and torch.equal(buf[33:], tail)
+
+
+def test_rows_that_overlap_are_refused(cuda_dev):
+    """Keys and values read back into each other, and rows that lie in a pool. Column
+    slices of one buffer lie apart, whatever their order."""
+    from ncmorph_b200 import _lib, kv_cache
+    from ncmorph_b200.kv_cache import KVCache
+    w = World(cuda_dev, torch.bfloat16, [9], [9], 1, 64, 16).fill()
+    buf = torch.zeros((9, 192), dtype=torch.bfloat16, device=cuda_dev)
+    at = w.starts([9])
+    flat = buf.view(-1)
+    shifted = torch.as_strided(flat, (4, 64), (128, 1), 8)
+    whole = kv_cache.gather(w.cache, at, w.table, rows=9)
+    for a, b in ((buf, buf), (buf[:, :64], buf[:, 32:96]), (buf[:, 120:184], buf[:, 64:192])):
+        with pytest.raises(_lib.NcmError):
+            kv_cache.gather(w.cache, at, w.table, out_k=a, out_v=b)
+    with pytest.raises(_lib.NcmError):  # rows of other strides over one range
+        kv_cache.gather(w.cache, w.starts([4]), w.table, out_k=buf[:4], out_v=shifted)
+    for a, b in ((buf[:, :64], buf[:, 64:]), (buf[:, 128:], buf[:, :64]), (buf[:, 64:128], buf[:, 128:]),
+                 (buf[:, 120:184], buf[:, 56:184])):  # (the first 64 columns of a slice are used)
+        k, v = kv_cache.gather(w.cache, at, w.table, out_k=a, out_v=b)
+        assert torch.equal(k[:, :64], whole[0]) and torch.equal(v[:, :64], whole[1])
+    # one below the other, the last row of the first beside the first of the second
+    k, v = torch.as_strided(flat, (5, 64), (128, 1), 0), torch.as_strided(flat, (5, 64), (128, 1), 4 * 128 + 64)
+    kv_cache.gather(w.cache, w.starts([5]), w.table, out_k=k, out_v=v)
+    assert torch.equal(k, whole[0][:5]) and torch.equal(v, whole[1][:5])
+    arena = torch.zeros((4, 1, 16, 64), dtype=torch.bfloat16, device=cuda_dev)
+    cache = KVCache(arena[:2], arena[2:])
+    apart, inside, edge = buf[:, :64], arena[1, 0, 4:13], torch.zeros((9, 64), dtype=torch.bfloat16, device=cuda_dev)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=cuda_dev)
+    for k, v in ((apart, inside), (inside, apart), (arena[3, 0, 7:], apart)):
+        with pytest.raises(_lib.NcmError):
+            kv_cache.append(cache, k, v, at, w.kv_lens, table)
+        with pytest.raises(_lib.NcmError):
+            kv_cache.gather(cache, at, table, out_k=k, out_v=v)
+    kv_cache.append(cache, edge, edge, at, w.kv_lens, table)  # the same rows twice, only read
