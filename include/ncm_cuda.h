@@ -627,21 +627,24 @@ NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, con
  * j when bit j % 32 of tree_mask[row * mask_words + j / 32] is set (its own bit
  * included; row = token_start[b] + i; missing words are zeros); tree_mask NULL: a chain, j <= i.
  *   out = sum_k softmax_k(scale q . k) v_k    lse = log sum_k exp(scale q . k)
- * per query head (head h reads kv head h / (heads / kv_heads), as
- * ncm_attention_bf16 does); a node that sees nothing gets zeros and -inf. q and
- * out [rows, heads * head_dim] bf16 (row strides in elements, multiples of 8;
- * 16-byte aligned, the two ranges apart), lse [rows, heads] f32 or NULL. max_nodes
- * bounds every sequence's new tokens (at most 1024; a sequence with more is skipped
- * with NCM_ERANGE), heads / kv_heads is at most 64 and max_nodes * heads /
- * kv_heads at most 32768. Scores (taken to be above -1e30), softmax and sums are
- * f32; for their product with the values the probabilities are rounded to bf16,
- * or, over codes and up to 32 rows of a kv head, to f16 (the values' scales, not
- * negative, included; half a step is 2^-11 of a term or 2^-32 of the row's largest). A new token's key or value that is not finite reaches only
- * the nodes that see it. How
- * the keys are split over the GPU (by all lengths of the call) changes a result by f32
- * roundings, and where such a one carries a probability over the border of its 16-bit
- * rounding, by that; it is the same on every run. `workspace` (16-byte aligned device memory) of
- * ncm_tree_attention_workspace bytes carries partial sums within the call. */
+ * per query head (head h reads kv head h / (heads / kv_heads), as ncm_attention_bf16
+ * does); a node that sees nothing gets zeros and -inf. q and out [rows, heads *
+ * head_dim] bf16 (row strides in elements, multiples of 8; 16-byte aligned, the two
+ * ranges apart), lse [rows, heads] f32 or NULL. max_nodes bounds every sequence's new
+ * tokens (at most 1024; a sequence with more is skipped with NCM_ERANGE) and picks the
+ * kernel, by max_nodes * heads / kv_heads rows of a kv head (tiles of 8 to 32, above
+ * them of 128): give it what the step has at most; heads / kv_heads is at most 64 and
+ * max_nodes * heads / kv_heads at most 32768. Scores (taken to be above -1e30), softmax
+ * and sums are f32 (values are taken to be below 2^80, a quantised row's largest above
+ * 2^-90 or 0: outside, sums may overflow and terms may be lost); for their product with
+ * the values the probabilities are rounded to bf16, or, over codes and up to 32 rows of
+ * a kv head, to f16 (the values' scales, not negative, included; half a step is 2^-11 of
+ * a term or 2^-32 of the row's largest). A new token's key or value that is not finite
+ * reaches only the nodes that see it. How the keys are split over the GPU (by all
+ * lengths of the call) changes a result by f32 roundings, and where such a one carries a
+ * probability over the border of its 16-bit rounding, by that; it is the same on every
+ * run. `workspace` (16-byte aligned device memory) of ncm_tree_attention_workspace bytes
+ * carries partial sums within the call. */
 NCM_API int ncm_tree_attention_workspace(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                          int32_t heads, int32_t max_nodes, uint64_t* bytes);
 NCM_API int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,

@@ -12,6 +12,10 @@ device tensors: sequence b's new tokens are rows token_start[b] ..
 token_start[b + 1], and kv_lens[b] counts its keys with them. Position p lives
 in slot p % page_size of page page_table[b, p // page_size].
 
+After drafted tokens are verified, ``append`` the accepted ones' rows again, from the
+step's own QKV rows and with ``kv_lens`` that count only them: they lie behind the context
+then, quantised once.
+
 ncmorph recomputes every position on each call (src/decoder.zig:50-58) and has no
 counterpart. There is no CPU path.
 """
@@ -143,7 +147,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     tokens, itself and the earlier new ones; with tree_mask [T, words] int32 those
     new tokens j whose bit j % 32 of word j / 32 is set. max_nodes bounds the new tokens of
     a sequence (at most 1024; a sequence with more is skipped and reported by
-    device.sync). scale defaults to head_dim ** -0.5. A token that sees nothing gets
+    device.sync) and picks the kernel, so give it what the step has at most. scale defaults to head_dim ** -0.5. A token that sees nothing gets
     zeros and -inf."""
     dev, hd = cache.device, cache.head_dim
     if heads is None:

@@ -1238,3 +1238,39 @@ def test_rows_that_overlap_are_refused(cuda_dev):
         with pytest.raises(_lib.NcmError):
             kv_cache.gather(cache, at, table, out_k=k, out_v=v)
     kv_cache.append(cache, edge, edge, at, w.kv_lens, table)  # the same rows twice, only read
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+@pytest.mark.parametrize("exponent", [-90, 80])
+@pytest.mark.parametrize("n,heads", [(1, 4), (8, 4), (40, 4)])
+def test_smallest_and_largest_values(cuda_dev, dtype, exponent, n, heads):
+    """Values at both ends of the documented range: nothing is lost or overflows."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, dtype, [2000, 60 + n], [n, n], 2, 64, 16, seed=n)
+    w.v = (w.v.double() * 2.0 ** exponent / w.v.double().abs().amax(1, keepdim=True)).to(torch.bfloat16)
+    w.fill()
+    q = torch.randn((w.T, heads * 64), generator=w.g).to(torch.bfloat16)
+    out, lse = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=n, return_lse=True)
+    o, l, to, tl = attend_ref(w, q, heads, None, 0.125)
+    to = to - 1e-37  # (an allowance for results near the end of f32's range, where these are not)
+    assert torch.all((out.cpu().double() - o).abs() <= to) and torch.all((lse.cpu().double() - l).abs() <= tl)
+
+
+@pytest.mark.parametrize("dtype", FORMATS)
+def test_accepted_tokens_are_appended_again(cuda_dev, dtype):
+    """After drafted tokens are verified, the accepted ones lie apart in the cache. Their rows are
+    still in the step's own arrays: appended again behind the context, they are the cache of
+    a context that was written token by token, with the same codes."""
+    from ncmorph_b200 import kv_cache
+    w = World(cuda_dev, dtype, [50, 33], [9, 7], 2, 64, 16).fill()
+    taken = [[0, 2, 5, 8], [1]]  # a path of each tree
+    rows = torch.tensor([w.at[b] + w.lens[b] - w.new[b] + i for b in range(2) for i in taken[b]])
+    lens = torch.tensor([w.lens[b] - w.new[b] + len(taken[b]) for b in range(2)], dtype=torch.int32, device=cuda_dev)
+    kv_cache.append(w.cache, w.k[rows].to(cuda_dev), w.v[rows].to(cuda_dev), w.starts([4, 1]), lens, w.table)
+    k, v = kv_cache.gather(w.cache, w.starts(lens.tolist()), w.table, rows=int(lens.sum()))
+    order = torch.cat([torch.cat([torch.arange(w.at[b], w.at[b] + w.lens[b] - w.new[b]), rows[4 * b:4 + b]]) for b in range(2)])
+    plain = World(cuda_dev, dtype, lens.tolist(), [1, 1], 2, 64, 16, seed=1)
+    plain.k, plain.v = w.k[order], w.v[order]
+    plain.fill()
+    k2, v2 = kv_cache.gather(plain.cache, w.starts(lens.tolist()), plain.table, rows=int(lens.sum()))
+    assert torch.equal(k, k2) and torch.equal(v, v2)
