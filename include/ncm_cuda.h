@@ -637,14 +637,14 @@ NCM_API int ncm_kv_cache_gather(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, con
  * max_nodes * heads / kv_heads at most 32768. Scores (taken to be above -1e30), softmax
  * and sums are f32 (values are taken to be below 2^80, a quantised row's largest above
  * 2^-90 or 0: outside, sums may overflow and terms may be lost); for their product with
- * the values the probabilities are rounded to bf16, or, over codes and up to 32 rows of
- * a kv head, to f16 (the values' scales, not negative, included; half a step is 2^-11 of
- * a term or 2^-32 of the row's largest). A new token's key or value that is not finite
- * reaches only the nodes that see it. How the keys are split over the GPU (by all
- * lengths of the call) changes a result by f32 roundings, and where such a one carries a
- * probability over the border of its 16-bit rounding, by that; it is the same on every
- * run. `workspace` (16-byte aligned device memory) of ncm_tree_attention_workspace bytes
- * carries partial sums within the call. */
+ * the values the probabilities are rounded to bf16, or, up to 32 rows of a kv head, to a
+ * sum of two bf16 values (2^-15 of a term), over codes to f16 (the values' scales, not
+ * negative, included; half a step is 2^-11 of a term or 2^-32 of the row's largest). A
+ * new token's key or value that is not finite reaches only the nodes that see it. How
+ * the keys are split over the GPU (by all lengths of the call) changes a result by f32
+ * roundings, and where such a one carries a probability over the border of its 16-bit
+ * rounding, by that; it is the same on every run. `workspace` (16-byte aligned device
+ * memory) of ncm_tree_attention_workspace bytes carries partial sums within the call. */
 NCM_API int ncm_tree_attention_workspace(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                          int32_t heads, int32_t max_nodes, uint64_t* bytes);
 NCM_API int ncm_tree_attention(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,

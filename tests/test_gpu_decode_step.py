@@ -1139,7 +1139,7 @@ def test_split_changes_no_rounding_of_probabilities(cuda_dev, dtype, n):
 
     Scores have the same bits. A probability is 2^(t - m), whose difference of up to 2^4 is
     rounded by 2^-21: 2^-20 apart, relative to itself, in two splits, so it falls on two sides
-    of a border of its rounding (steps of 2^-8 or, over codes, 2^-11, relative to it) with a chance
+    of a border of its rounding (steps of 2^-8 for one bf16 value or, over codes, 2^-11, relative to it) with a chance
     of 2^-12 or 2^-9, and is then a step off. For an output, a sum of many of random signs,
     that is sqrt(2^-12) 2^-8 or sqrt(2^-9) 2^-11 of itself, about 2^-14 or 2^-15.5; the f32 sums'
     order is below that. It takes another bf16 (steps of 2^-8 to 2^-7) with a chance of 1.6 % or 0.6 %.
@@ -1274,3 +1274,33 @@ def test_accepted_tokens_are_appended_again(cuda_dev, dtype):
     plain.fill()
     k2, v2 = kv_cache.gather(plain.cache, w.starts(lens.tolist()), plain.table, rows=int(lens.sum()))
     assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+@pytest.mark.parametrize("lens", [[1, 2, 5], [12, 31, 79], [200, 1500, 3]])
+@pytest.mark.parametrize("n,heads,hd", [(1, 1, 64), (1, 16, 64), (1, 16, 128), (3, 4, 64), (3, 4, 128), (4, 8, 64), (4, 8, 128)])
+def test_probabilities_over_a_bf16_cache(cuda_dev, lens, n, heads, hd):
+    """Up to 32 rows of a kv head: probabilities are two bf16 values. The first is cut off, up to
+    2^-7 of a term below it, and half a step of the second, the rest, is 2^-8 of that; with
+    the 2^-20 that are added, 2^-15 + 2^-20 of a term. So little but the output's own rounding is
+    seen, and a row that sees one key returns its value: half of a bf16 step is 2^-9 of it or more."""
+    from ncmorph_b200 import kv_cache
+    new = [min(n, x) for x in lens]
+    w = World(cuda_dev, torch.bfloat16, lens, new, 1, hd, 16, seed=n * hd).fill()
+    q = torch.randn((w.T, heads * hd), generator=w.g).to(torch.bfloat16)
+    out = kv_cache.tree_attention(q.to(cuda_dev), w.cache, w.start, w.kv_lens, w.table, max_nodes=n).cpu()
+    o, _, to, _ = attend_ref(w, q, heads, None, hd ** -0.5)
+    k0 = int(w.at[0])
+    if lens[0] == new[0]:  # its first new token sees itself only
+        assert torch.equal(out[0].view(heads, hd), w.v[k0].expand(heads, hd))
+    # check_attention's tolerance holds 2^-8 of every term for P
+    K, V = w.held(w.k), w.held(w.v)
+    row = 0
+    for b, m in enumerate(new):
+        k, v = K[w.at[b]:w.at[b] + lens[b], 0], V[w.at[b]:w.at[b] + lens[b], 0]
+        t = torch.einsum("nhd,ld->nhl", q[row:row + m].double().view(m, heads, hd), k) * hd ** -0.5
+        seen = torch.arange(lens[b])[None] <= lens[b] - m + torch.arange(m)[:, None]
+        p = torch.softmax(t.masked_fill(~seen[:, None], -math.inf), -1)
+        spread = torch.einsum("nhl,ld->nhd", p, v.abs()).reshape(m, -1)
+        tol = to[row:row + m] - (BF - 2.0 ** -15 - 2.0 ** -20) * spread
+        assert torch.all((out[row:row + m].double() - o[row:row + m]).abs() <= tol)
+        row += m
