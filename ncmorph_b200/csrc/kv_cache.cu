@@ -13,9 +13,11 @@
 // arithmetic, ties included, without a division per value.
 //
 // Bound: memory; no value is used twice. 16 thousand tokens of 8 heads of 128: written
-// as e4m3 in 26 us (3.9 TB/s moved: the conversions take half of the issue slots, and 60
-// registers leave four blocks an SM), read back in 18 us. Contexts of 16 sequences of up
-// to 16384 tokens, 8 heads of 64, int8: read back in 52.5 us, 5.5 TB/s, 0.84 of a copy.
+// as bf16 in 26.3 us (5.1 TB/s moved), as int8 or e4m3 in 26.7 (3.8 TB/s): the same time
+// for fewer bytes. Rows are asked for once their slots are known, and 44 (60) registers leave
+// five (four) blocks an SM, so too few bytes are on their way; ALU and issue slots are half
+// idle. Read back in 19-22 us. Contexts of 16 sequences of up to 16384 tokens, 8 heads of 64,
+// int8: read back in 53 us, 5.4 TB/s, 0.83 of a copy.
 #include <algorithm>
 
 #include "kv_cache.cuh"

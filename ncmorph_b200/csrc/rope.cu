@@ -7,8 +7,9 @@
 // Bound: memory. A rotated element is read and written once (4 bytes); the
 // table rows add 4 r bytes per token and are shared by its heads through L1.
 // 16384 rows of 40 heads of 128 with 64 columns rotated as neighbours: 56 us, 6.06
-// TB/s moved, 0.92 of a copy. 48 rows of 40 heads of 64: 1.6 us beside its neighbours
-// in a graph.
+// TB/s moved, 0.92 of a copy; as halves 62 us, 5.5 TB/s. Whole heads as halves, the decoder's
+// layout: 28.2 us for 40 heads of 64, 6.1 TB/s, 0.93 of a copy, 55.9 us for 40 of 128. 48 rows
+// of 40 heads of 64: 1.6 us beside its neighbours in a graph.
 #include <algorithm>
 
 #include "internal.h"
@@ -45,8 +46,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // the rotated columns: one piece copied); otherwise one pair, or one column
 // copied. A thread keeps its unit (blockIdx.y picks the part of the row) and
 // walks over the block's tokens, BATCH of them loaded before the first is used: two
-// are enough at the occupancy that 32 registers allow (us of 2, 3, 4 and 8 for the rows
-// above: 56, 58, 57 and 84). Rows pass the caches by (__ldcs, __stcs: 58 without).
+// are enough (us of 2, 3, 4 and 8 for the neighbours above: 56, 58, 57 and 84), at 32
+// registers a thread for neighbours and 52 for halves, whose unit is two pieces. Rows pass the caches by (__ldcs, __stcs: 58 without).
 template <bool VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
   pdl_wait();

@@ -37,8 +37,9 @@
 // Bound: the cache's bytes with few rows (single tokens of 32 sequences of up to
 // 32768 tokens, 32 query over 8 kv heads of 64, int8: 70 us, 5.6 TB/s, 0.85 of a
 // copy), the issue slots of softmax and conversion with 32 rows (eight tokens of eight
-// sequences, int8: 34 us, 1.6 TB/s). A short context (4 sequences of 200 tokens) takes
-// 5.7 us: one launch, and a chain of four loads.
+// sequences, int8: 33 us, 1.6 TB/s, a quarter of a copy; every warp turns every code into
+// f16 for its few rows, and 255 registers leave two CTAs an SM). A short context (4 sequences
+// of 200 tokens) takes 5.7 us: one launch, and a chain of four loads.
 //
 // Split: items are cut into units of 128 keys, and every CTA of one wave takes
 // the same number of consecutive units (beginning an item counts as three more),
@@ -579,7 +580,9 @@ __global__ void __launch_bounds__(32 * RG * KG, TreeShape<HD, FMT, NT, RG, KG>::
 // Adds up the partial sums of a row of an item (blockIdx.x: sequence and kv
 // head, blockIdx.y: 4 / WPR rows of the sequence's rows), in an order that the
 // split alone decides. WPR warps share a row: all four of the block where there are few
-// rows (kManyRows), otherwise one. What the caller
+// rows (kManyRows), otherwise one. Each row's warps look all sequences up for their places, which
+// grows with rows x sequences: 4 of the 14 us of 32 sequences of up to 1600 keys, 265 of
+// 600 us of 2048. What the caller
 // gave is read before the wait: the attention kernel does not let this one start
 // ahead of its own end, and the kernels in front of both are done by then.
 constexpr int kMaxParts = 2048;  // CTAs of the attention kernel at most
@@ -720,9 +723,9 @@ struct Variants {
 
 // Rows of one kv head that stay with the mma.sync kernel. More go to the tcgen05
 // kernel, whose tiles have 128 rows. us of both, mma.sync / tcgen05 (eight
-// sequences of 1 to 16 thousand tokens, 8 kv heads): 32 rows, bf16: 29 / 40 at
-// head_dim 64, 44 / 63 at 128, int8: 34 / 44 and 48 / 65; 48 rows: 40 / 41, 67 / 64,
-// 48 / 45 and 78 / 69; 64 rows: 41 / 42, 68 / 65, 49 / 45 and 79 / 70.
+// sequences of 1 to 16 thousand tokens, 8 kv heads): 32 rows, bf16: 32 / 40 at
+// head_dim 64, 49 / 63 at 128, int8: 33 / 44 and 48 / 65; 48 rows (bf16 with P as one
+// value): 40 / 41, 67 / 64, 48 / 45 and 78 / 69; 64 rows: 41 / 42, 68 / 65, 49 / 45 and 79 / 70.
 constexpr int64_t kFewRows = 32;
 Variant pick(const ncm_kv_cache_t* c, int64_t rows, int* index) {
   const bool wide = c->head_dim == 128;
