@@ -47,7 +47,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // copied. A thread keeps its unit (blockIdx.y picks the part of the row) and
 // walks over the block's tokens, BATCH of them loaded before the first is used: two
 // are enough (us of 2, 3, 4 and 8 for the neighbours above: 56, 58, 57 and 84), at 32
-// registers a thread for neighbours and 52 for halves, whose unit is two pieces. Rows pass the caches by (__ldcs, __stcs: 58 without).
+// registers a thread for neighbours and 52 for halves, whose unit is two pieces. Rows pass
+// the caches by (__ldcs, __stcs: 58 without).
 template <bool VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
   pdl_wait();

@@ -147,8 +147,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, token_start: torch.Tensor, k
     tokens, itself and the earlier new ones; with tree_mask [T, words] int32 those
     new tokens j whose bit j % 32 of word j / 32 is set. max_nodes bounds the new tokens of
     a sequence (at most 1024; a sequence with more is skipped and reported by
-    device.sync) and picks the kernel, so give it what the step has at most. scale defaults to head_dim ** -0.5. A token that sees nothing gets
-    zeros and -inf."""
+    device.sync) and picks the kernel, so give it what the step has at most. scale
+    defaults to head_dim ** -0.5. A token that sees nothing gets zeros and -inf."""
     dev, hd = cache.device, cache.head_dim
     if heads is None:
         if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] % hd:
